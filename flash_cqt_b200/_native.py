@@ -54,6 +54,39 @@ class CqtSlices(ctypes.Structure):
                 ("slices", ctypes.c_int32), ("window", ctypes.c_void_p)]
 
 
+class CqtAdamwTensor(ctypes.Structure):
+    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p),
+                ("master", ctypes.c_void_p), ("exp_avg", ctypes.c_void_p),
+                ("exp_avg_sq", ctypes.c_void_p), ("exp_avg_scale", ctypes.c_void_p),
+                ("exp_avg_sq_scale", ctypes.c_void_p), ("step", ctypes.c_void_p),
+                ("numel", ctypes.c_int64), ("dtype", ctypes.c_int32),
+                ("ordinal", ctypes.c_int32)]
+
+
+class CqtAdamwArgs(ctypes.Structure):
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double),
+                ("beta2", ctypes.c_double), ("eps", ctypes.c_double),
+                ("weight_decay", ctypes.c_double), ("max_norm", ctypes.c_double),
+                ("lr_dev", ctypes.c_void_p), ("use_norm", ctypes.c_int32),
+                ("seed", ctypes.c_uint32)]
+
+
+class CqtCache(ctypes.Structure):
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+                ("length", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+                ("rows", ctypes.c_int32), ("capacity", ctypes.c_int32),
+                ("format", ctypes.c_int32), ("ngroups", ctypes.c_int32),
+                ("group_count", _i32p), ("group_len", _i32p)]
+
+
+class CqtCachePart(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_int64),
+                ("slice_stride", ctypes.c_int64), ("band_stride", ctypes.c_int64)]
+
+
+CQT_F32, CQT_BF16, CQT_F16 = 0, 1, 2
+CQT_CACHE_INT8, CQT_CACHE_E4M3 = 0, 1
+
 _lib = None
 _lock = threading.Lock()
 
@@ -127,6 +160,17 @@ def lib():
             for nm in ("cqt_sliced_analysis", "cqt_sliced_adj_synthesis",
                        "cqt_sliced_synthesis", "cqt_sliced_adj_analysis"):
                 getattr(L, nm).restype = ci
+            atp = ctypes.POINTER(CqtAdamwTensor)
+            L.cqt_adamw_workspace_bytes.argtypes = [ci]
+            L.cqt_adamw_workspace_bytes.restype = sz
+            L.cqt_grad_norm.argtypes = [atp, ci, vp, vp, sz, vp]
+            L.cqt_adamw_step.argtypes = [atp, ci, ci, ctypes.POINTER(CqtAdamwArgs), vp, sz, vp]
+            cp, pp = ctypes.POINTER(CqtCache), ctypes.POINTER(CqtCachePart)
+            L.cqt_cache_append.argtypes = [cp, pp, ci, vp, vp]
+            L.cqt_cache_window.argtypes = [cp, pp, ci, vp, ci, vp]
+            for nm in ("cqt_grad_norm", "cqt_adamw_step", "cqt_cache_append",
+                       "cqt_cache_window"):
+                getattr(L, nm).restype = ci
             _lib = L
     return _lib
 
@@ -142,7 +186,9 @@ def exported_symbols():
             "cqt_sliced_adj_synthesis", "cqt_halo_create", "cqt_halo_connect",
             "cqt_halo_send", "cqt_halo_recv_add", "cqt_halo_waits", "cqt_halo_free",
             "cqt_wait_timeouts", "cqt_workspace_waits",
-            "cqt_debug_expire_waits", "cqt_last_error", "cqt_version"]
+            "cqt_debug_expire_waits", "cqt_adamw_workspace_bytes", "cqt_grad_norm",
+            "cqt_adamw_step", "cqt_cache_append", "cqt_cache_window",
+            "cqt_last_error", "cqt_version"]
 
 
 WS_HEADER = 256   # bytes at the front of a workspace: the wait-status word

@@ -3,6 +3,7 @@
 // kernels on the caller's stream and reports launch errors; none allocates
 // or synchronises.
 #include <atomic>
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
@@ -935,6 +936,215 @@ int cqt_sliced_adj_analysis(const cqt_tables* t, const float* gcoef, const cqt_s
     if (!sl || !sl->window)
         return fail(CQT_ERR_ARG, "the transpose of the sliced analysis needs the window");
     return sliced_inv(t, 1, gcoef, sl, sl->window, gx, ws, ws_bytes, stream);
+}
+
+// ---- AdamW over many tensors (optim.cu)
+// workspace: [0] the ticket, [8] the norm in 64 bits, [256] one partial sum per
+// CTA of each launch
+static size_t adamw_ws(int count) {
+    const size_t launches = ((size_t)count + kOptTensors - 1) / kOptTensors;
+    return kWsHeader + launches * kOptCtas * sizeof(double);
+}
+
+size_t cqt_adamw_workspace_bytes(int count) { return count < 0 ? 0 : adamw_ws(count); }
+
+static int check_adamw_ws(int count, void* ws, size_t bytes) {
+    if (count < 0) return fail(CQT_ERR_ARG, "negative tensor count");
+    if (!ws || bytes < adamw_ws(count))
+        return fail(CQT_ERR_ARG, "workspace missing or smaller than cqt_adamw_workspace_bytes");
+    if ((uintptr_t)ws & 15u) return fail(CQT_ERR_ARG, "workspace not 16-byte aligned");
+    return CQT_OK;
+}
+
+static bool opt_type(int32_t d) { return d == CQT_F32 || d == CQT_BF16 || d == CQT_F16; }
+
+// the next tensors of the list that hold elements, at most kOptTensors of them
+static int take_tensors(const cqt_adamw_tensor* in, int count, int* at, OptTensor* out, int* n,
+                        bool grads_only, int bits) {
+    static_assert(kOptF32 == CQT_F32 && kOptBf16 == CQT_BF16 && kOptF16 == CQT_F16, "types");
+    long long chunks = 0;
+    *n = 0;
+    for (; *at < count && *n < kOptTensors; ++*at) {
+        const cqt_adamw_tensor& x = in[*at];
+        if (x.numel < 0 || !opt_type(x.dtype))
+            return fail(CQT_ERR_ARG, "bad tensor (numel >= 0, a known dtype)");
+        if (x.numel == 0) continue;
+        const uintptr_t item = x.dtype == CQT_F32 ? 4 : 2;
+        if (!x.grad || (uintptr_t)x.grad % item)
+            return fail(CQT_ERR_ARG, "null or misaligned gradient");
+        uintptr_t low = (uintptr_t)x.grad;
+        bool codes = true;
+        if (!grads_only) {
+            const uintptr_t p = (uintptr_t)x.param, ma = (uintptr_t)x.master;
+            const uintptr_t m = (uintptr_t)x.exp_avg, v = (uintptr_t)x.exp_avg_sq;
+            if (!p || !m || !v || !x.step || p % item || ma % 4 || (uintptr_t)x.step % 8)
+                return fail(CQT_ERR_ARG, "null or misaligned parameter, moments or step");
+            if (x.master && x.dtype == CQT_F32)
+                return fail(CQT_ERR_ARG, "a master copy is for 16-bit parameters");
+            if (bits == 8 ? (!x.exp_avg_scale || !x.exp_avg_sq_scale) : ((m | v) % 4) != 0)
+                return fail(CQT_ERR_ARG, "null scales or misaligned moments");
+            low |= p | ma | (bits == 8 ? 0 : m | v);
+            codes = bits == 32 || ((m | v) & 7u) == 0;
+        }
+        chunks += opt_chunks(x.numel);
+        if (chunks >= (1LL << 31)) return fail(CQT_ERR_ARG, "too many elements in one call");
+        OptTensor& o = out[(*n)++];
+        o.p = x.param;
+        o.g = x.grad;
+        o.master = x.master;
+        o.m = x.exp_avg;
+        o.v = x.exp_avg_sq;
+        o.ms = x.exp_avg_scale;
+        o.vs = x.exp_avg_sq_scale;
+        o.step = reinterpret_cast<long long*>(x.step);
+        o.n = x.numel;
+        o.chunk0 = 0;
+        o.dtype = (short)x.dtype;
+        o.vec = (low & 15u) == 0 && codes;
+        o.ordinal = x.ordinal;
+    }
+    return CQT_OK;
+}
+
+int cqt_grad_norm(const cqt_adamw_tensor* tensors, int count, float* norm, void* workspace,
+                  size_t workspace_bytes, void* stream) {
+    if (int rc = check_adamw_ws(count, workspace, workspace_bytes)) return rc;
+    if (count > 0 && !tensors) return fail(CQT_ERR_ARG, "null tensors");
+    char* ws = static_cast<char*>(workspace);
+    double* sum = reinterpret_cast<double*>(ws + 8);
+    float* out = norm ? norm : reinterpret_cast<float*>(ws + 16);
+    OptTensor part[kOptTensors];
+    int at = 0, n = 0, first = 0;
+    do {   // a list without elements has the norm 0: one launch in any case
+        if (int rc = take_tensors(tensors, count, &at, part, &n, true, 32)) return rc;
+        bool last = true;
+        for (int i = at; i < count; ++i) last = last && tensors[i].numel == 0;
+        const cudaError_t e = launch_grad_norm(
+            part, n, reinterpret_cast<double*>(ws + kWsHeader), &first, last,
+            reinterpret_cast<unsigned*>(ws), sum, out, static_cast<cudaStream_t>(stream));
+        if (e != cudaSuccess) return cuda_fail(e, "grad_norm launch");
+        if (last) break;
+    } while (at < count);
+    return CQT_OK;
+}
+
+int cqt_adamw_step(const cqt_adamw_tensor* tensors, int count, int state_bits,
+                   const cqt_adamw_args* a, void* workspace, size_t workspace_bytes,
+                   void* stream) {
+    if (int rc = check_adamw_ws(count, workspace, workspace_bytes)) return rc;
+    if (!a || (count > 0 && !tensors)) return fail(CQT_ERR_ARG, "null tensors or arguments");
+    if (state_bits != 8 && state_bits != 32)
+        return fail(CQT_ERR_ARG, "state_bits must be 8 or 32");
+    if (!(a->beta1 >= 0 && a->beta1 < 1 && a->beta2 >= 0 && a->beta2 < 1) || !(a->eps >= 0))
+        return fail(CQT_ERR_ARG, "betas must lie in [0, 1) and eps must not be negative");
+    if (a->use_norm && !(a->max_norm > 0)) return fail(CQT_ERR_ARG, "max_norm must be positive");
+    OptArgs o{};
+    o.lr = a->lr;
+    o.wd = a->weight_decay;
+    o.lb1 = std::log2(a->beta1);
+    o.lb2 = std::log2(a->beta2);
+    o.lr_dev = a->lr_dev;
+    o.norm = a->use_norm
+                 ? reinterpret_cast<const double*>(static_cast<char*>(workspace) + 8) : nullptr;
+    o.max_norm = a->max_norm;
+    o.ticket = static_cast<unsigned*>(workspace);
+    o.b1 = (float)a->beta1;
+    o.omb1 = (float)(1.0 - a->beta1);
+    o.b2 = (float)a->beta2;
+    o.omb2 = (float)(1.0 - a->beta2);
+    o.eps = (float)a->eps;
+    o.seed_key = a->seed;
+    OptTensor part[kOptTensors];
+    for (int at = 0, n = 0; at < count;) {
+        if (int rc = take_tensors(tensors, count, &at, part, &n, false, state_bits)) return rc;
+        if (n == 0) break;
+        const cudaError_t e =
+            launch_adamw(part, n, state_bits, o, static_cast<cudaStream_t>(stream));
+        if (e != cudaSuccess) return cuda_fail(e, "adamw launch");
+    }
+    return CQT_OK;
+}
+
+// ---- coefficient cache (coefcache.cu)
+static int cache_args(const cqt_cache* c, const cqt_cache_part* parts, int slices, int item,
+                      bool write, CacheStore* st, CacheGroups* gr) {
+    if (!c || !parts) return fail(CQT_ERR_ARG, "null cache or parts");
+    if (c->rows < 0 || c->capacity < 1 || slices < 0)
+        return fail(CQT_ERR_ARG, "bad cache (rows >= 0, capacity >= 1) or slice count");
+    if (c->format != CQT_CACHE_INT8 && c->format != CQT_CACHE_E4M3)
+        return fail(CQT_ERR_ARG, "unknown cache format");
+    if (c->ngroups < 1 || c->ngroups > kMaxGroups || !c->group_count || !c->group_len)
+        return fail(CQT_ERR_ARG, "bad group layout (1 to 16 groups)");
+    if (!c->workspace || (uintptr_t)c->workspace % 16)
+        return fail(CQT_ERR_ARG, "workspace missing or not 16-byte aligned");
+    if (c->rows > 0 && (!c->codes || !c->scales || !c->length || (uintptr_t)c->codes % 16 ||
+                        (uintptr_t)c->length % 8))
+        return fail(CQT_ERR_ARG, "null or misaligned codes, scales or lengths");
+    long long off = 0;
+    gr->count = c->ngroups;
+    gr->wide = 1;
+    for (int g = 0; g < kMaxGroups; ++g) {
+        gr->data[g] = nullptr;
+        gr->row[g] = gr->slice[g] = gr->band[g] = 0;
+        gr->off[g] = INT32_MAX;
+        gr->shift[g] = 0;
+    }
+    for (int g = 0; g < c->ngroups; ++g) {
+        const int32_t b = c->group_count[g], m = c->group_len[g];
+        if (b < 1 || b > kMaxBands || m < 16 || m > (1 << 20) || (m & (m - 1)))
+            return fail(CQT_ERR_ARG, "a group needs bands and a block length 2^k >= 16");
+        const cqt_cache_part& p = parts[g];
+        gr->data[g] = p.data;
+        gr->row[g] = p.row_stride;
+        gr->slice[g] = p.slice_stride;
+        gr->band[g] = p.band_stride;
+        gr->off[g] = (int)off;
+        while ((1 << gr->shift[g]) < m) ++gr->shift[g];
+        off += (long long)b * m;
+        if (off >= (1LL << 30)) return fail(CQT_ERR_ARG, "too many coefficients in a slice");
+        if (c->rows > 0 && slices > 0 && (!p.data || (uintptr_t)p.data % 8))
+            return fail(CQT_ERR_ARG, "null or misaligned coefficients");
+        const long long strides = p.row_stride | p.slice_stride | p.band_stride;
+        if ((uintptr_t)p.data % 16 || (strides * item) % 16) gr->wide = 0;
+    }
+    if (!write && !gr->wide)
+        return fail(CQT_ERR_ARG, "window outputs and their strides must be 16-byte aligned");
+    st->codes = static_cast<unsigned char*>(c->codes);
+    st->scales = c->scales;
+    st->length = reinterpret_cast<long long*>(c->length);
+    st->ticket = static_cast<unsigned*>(c->workspace);
+    st->rows = c->rows;
+    st->capacity = c->capacity;
+    st->ncoef = (int)off;
+    st->int8 = c->format == CQT_CACHE_INT8;
+    // bounded before they are multiplied
+    if ((long long)slices * c->rows >= (1LL << 31) || cache_unit_count(*st, slices) >= (1LL << 31))
+        return fail(CQT_ERR_ARG, "too many slices in one call");
+    return CQT_OK;
+}
+
+int cqt_cache_append(const cqt_cache* c, const cqt_cache_part* parts, int slices,
+                     const int64_t* counts, void* stream) {
+    CacheStore st;
+    CacheGroups gr;
+    if (int rc = cache_args(c, parts, slices, 8, true, &st, &gr)) return rc;
+    const cudaError_t e =
+        launch_cache_append(st, gr, slices, reinterpret_cast<const long long*>(counts),
+                            static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? CQT_OK : cuda_fail(e, "cache append launch");
+}
+
+int cqt_cache_window(const cqt_cache* c, const cqt_cache_part* parts, int slices,
+                     const int64_t* ends, int dtype, void* stream) {
+    CacheStore st;
+    CacheGroups gr;
+    if (!opt_type(dtype)) return fail(CQT_ERR_ARG, "unknown output type");
+    if (int rc = cache_args(c, parts, slices, dtype == CQT_F32 ? 8 : 4, false, &st, &gr))
+        return rc;
+    const cudaError_t e =
+        launch_cache_window(st, gr, slices, reinterpret_cast<const long long*>(ends), dtype,
+                            static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? CQT_OK : cuda_fail(e, "cache window launch");
 }
 
 }  // extern "C"

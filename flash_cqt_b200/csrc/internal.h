@@ -232,4 +232,76 @@ cudaError_t launch_bands_inv(CoefPtr in, const InvTab& tab, int which, const Ban
 int band_twiddle_count();
 void band_twiddle_rows(float2* out, const float2* w2048);
 
+
+// ---------------------------------------------------------------------------
+// AdamW over many tensors (optim.cu)
+constexpr int kOptBlock = 256;     // elements that share a scale (8-bit moments)
+constexpr int kOptTensors = 360;   // tensors in one launch (32 KB of kernel parameters)
+constexpr int kOptCtas = 148 * 4;  // CTAs of one launch at most
+enum OptType { kOptF32 = 0, kOptBf16 = 1, kOptF16 = 2 };
+
+struct OptTensor {
+    void* p;               // parameter, n values of `dtype`
+    const void* g;         // gradient, the same type
+    float* master;         // 32-bit copy of a 16-bit parameter, or null
+    void* m;               // first moment: float32, or e4m3 codes
+    void* v;               // second moment: float32, or e5m2 codes
+    unsigned char* ms;     // scale bytes of m and v, one per kOptBlock elements
+    unsigned char* vs;
+    long long* step;       // steps taken so far (device)
+    long long n;
+    unsigned chunk0;       // first chunk of the tensor (filled in for the launch)
+    short dtype;           // OptType
+    short vec;             // every array is aligned for 8 values at once
+    int ordinal;           // the tensor's number in the rounding hash
+};
+
+struct OptArgs {
+    double lr, wd, lb1, lb2;   // lb: log2 of the betas
+    const float* lr_dev;       // not null: the rate is read from the device
+    const double* norm;        // not null: gradients are scaled to max_norm
+    double max_norm;
+    unsigned* ticket;          // zero between launches
+    float b1, omb1, b2, omb2, eps;
+    unsigned seed_key;
+};
+
+// one launch over at most kOptTensors tensors
+cudaError_t launch_adamw(const OptTensor* t, int count, int bits, OptArgs a, cudaStream_t s);
+// one launch of norm = sqrt(sum of the squares of all gradients): the sums of
+// its CTAs go to partial[*first ...], and the last launch adds them all up
+cudaError_t launch_grad_norm(const OptTensor* t, int count, double* partial, int* first, bool last,
+                             unsigned* ticket, double* norm, float* norm32, cudaStream_t s);
+long long opt_chunks(long long n);   // chunks of work of n elements
+
+// ---------------------------------------------------------------------------
+// coefficient cache (coefcache.cu)
+struct CacheStore {
+    unsigned char* codes;      // [rows][capacity][ncoef][2]
+    unsigned char* scales;     // [rows][capacity][ncoef / 16], exponent + 127
+    long long* length;         // [rows] slices written so far
+    unsigned* ticket;          // zero between launches
+    int rows, capacity, ncoef;
+    int int8;                  // 1: int8 codes, 0: e4m3
+};
+
+// the groups' tensors: element (row, slice, band, t) of group g lies at
+// data[g] + row * row[g] + slice * slice[g] + band * band[g] + t, in complex
+// values
+struct CacheGroups {
+    void* data[kMaxGroups];
+    long long row[kMaxGroups], slice[kMaxGroups], band[kMaxGroups];
+    int off[kMaxGroups];       // heap offset of the group
+    int shift[kMaxGroups];     // log2 of its block length
+    int count;
+    int wide;                  // every quad is 16-byte aligned
+};
+
+// units of work of a call (the caller keeps them below 2^31)
+long long cache_unit_count(const CacheStore& st, long long slices);
+cudaError_t launch_cache_append(const CacheStore& st, const CacheGroups& gr, int slices,
+                                const long long* counts, cudaStream_t s);
+cudaError_t launch_cache_window(const CacheStore& st, const CacheGroups& gr, int slices,
+                                const long long* ends, int dtype, cudaStream_t s);
+
 }  // namespace fcqt

@@ -1,0 +1,337 @@
+"""``AdamW``: the optimizer's step of a training loop around the transform.
+
+The update of every tensor -- and, with ``max_norm``, the global gradient norm
+that scales the gradients -- runs in the library's kernels (``csrc/optim.cu``):
+one launch for up to 360 tensors, moments in 32 or in 8 bits, nothing read
+back to the host.  Counts of steps live on the device, so a captured graph that
+holds a step advances them with every replay.
+
+    opt = AdamW([x], lr=1e-2, max_norm=1.0)
+    loss = t.mse_loss(*t.fwd(x), target)
+    loss.backward()
+    opt.step()
+"""
+import ctypes
+
+import torch
+
+from . import _native
+from .engine import _raw_stream_of
+
+BLOCK = 256   # elements that share a scale in the 8-bit moments
+_TYPES = {torch.float32: _native.CQT_F32, torch.bfloat16: _native.CQT_BF16,
+          torch.float16: _native.CQT_F16, torch.complex64: _native.CQT_F32}
+
+
+def _dense(t):
+    """whether the elements fill one stretch of memory, in any order of dims"""
+    want = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def _same_order(a, b):
+    """whether element i of a's memory is element i of b's (both dense)"""
+    return all(x == y for x, y, n in zip(a.stride(), b.stride(), a.shape) if n != 1)
+
+
+def _reals(t):
+    return t.numel() * (2 if t.is_complex() else 1)
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW over all parameters at once.
+
+    With t the number of steps that a parameter has taken (one with no gradient
+    is left out of a step), per real element::
+
+        g' = g * min(1, max_norm / (norm + 1e-6))      norm over all parameters
+        m  = b1 m + (1 - b1) g'
+        v  = b2 v + (1 - b2) g'^2
+        p  = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+
+    in 32 bits.  Real and imaginary parts of a complex64 parameter are elements
+    of their own.  float32, bfloat16, float16 and complex64 parameters on one
+    CUDA device, dense in memory (in any order of dimensions).  A gradient in
+    another order than its parameter is copied first.
+
+    ``lr`` may be a 0-dim float32 tensor on the device (read by the kernel, so a
+    captured step follows it); any other number is fixed when a graph is
+    captured.
+
+    ``state_bits=8`` holds the moments in 8 bits: ``exp_avg`` as float8_e4m3fn
+    and ``exp_avg_sq`` as float8_e5m2 values in the parameter's memory order,
+    256 of which share a power-of-two scale (``exp_avg_scale``,
+    ``exp_avg_sq_scale``, float8_e8m0fnu).  They are rounded stochastically by a
+    hash of (``seed``, t, the parameter's number, element): the same run gives
+    the same bits.  ``master=True`` keeps a 32-bit copy of a 16-bit parameter,
+    which is then its rounding; without it a 16-bit parameter loses updates
+    below half a step of its type.  Both may differ between parameter groups.
+
+    ``max_norm`` scales the gradients as they are read (they stay as they are
+    in memory); ``grad_norm`` is the norm before scaling, a 0-dim float32
+    device tensor that every step overwrites, or None without ``max_norm``.
+    Gradients that are not finite go through as the formulas say.
+
+    Steps of one optimizer must be ordered on one stream at a time.  State is
+    made at a parameter's first step; before a step is captured it has to be
+    there (``init_state()``, or a step).  State is replaced through
+    ``load_state_dict`` (which also takes the state of ``torch.optim.AdamW``).
+    """
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *,
+                 state_bits=32, master=False, max_norm=None, seed=0):
+        if max_norm is not None and not float(max_norm) > 0:
+            raise ValueError(f"max_norm must be positive, got {max_norm}")
+        self.max_norm = None if max_norm is None else float(max_norm)
+        self.seed = int(seed) & 0xffffffff
+        self._reset()
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
+                                      state_bits=state_bits, master=master))
+
+    def _reset(self):
+        self._dev = self._ws = self.grad_norm = None
+        self._retired = []
+
+    def __getstate__(self):
+        return dict(super().__getstate__(), max_norm=self.max_norm, seed=self.seed)
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._reset()
+        for g in self.param_groups:
+            self._dev = g["params"][0].device if g["params"] else self._dev
+
+    # ------------------------------------------------------------------ checks
+    @staticmethod
+    def _check_options(g):
+        lr, (b1, b2) = g["lr"], g["betas"]
+        if torch.is_tensor(lr):
+            if lr.numel() != 1:
+                raise ValueError(f"a tensor lr must hold one number, got {tuple(lr.shape)}")
+            if lr.device.type == "cuda" and lr.dtype != torch.float32:
+                raise TypeError(f"a device lr must be float32, got {lr.dtype}")
+        elif not float(lr) >= 0:
+            raise ValueError(f"lr must not be negative, got {lr}")
+        if not (0 <= b1 < 1 and 0 <= b2 < 1):
+            raise ValueError(f"betas must lie in [0, 1), got {(b1, b2)}")
+        if not g["eps"] >= 0 or not g["weight_decay"] >= 0:
+            raise ValueError("eps and weight_decay must not be negative")
+        if g["state_bits"] not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {g['state_bits']}")
+
+    def add_param_group(self, group):
+        group = dict(group)
+        params = group["params"]
+        params = [params] if torch.is_tensor(params) else list(params)
+        group["params"] = params
+        self._check_options({**self.defaults, **group})
+        tensors = [p[1] if isinstance(p, tuple) else p for p in params]
+        spans = [s for g in self.param_groups for p in g["params"] for s in self._span(p)]
+        for p in tensors:
+            if not torch.is_tensor(p):
+                raise TypeError(f"parameters must be tensors, got {type(p).__name__}")
+            if p.dtype not in _TYPES:
+                raise TypeError("parameters must be float32, bfloat16, float16 or complex64, "
+                                f"got {p.dtype}")
+            if p.is_conj() or p.is_neg() or not _dense(p):
+                raise ValueError("parameters must be dense in memory (no gaps, no elements "
+                                 "that share a place, no lazy conjugate)")
+            if p.device.type != "cuda":
+                raise RuntimeError(f"the optimizer step runs on CUDA devices only, got {p.device} "
+                                   "(there is no CPU fallback)")
+            if self._dev is not None and p.device != self._dev:
+                raise ValueError(f"parameters must be on one device: {p.device}, {self._dev}")
+            self._dev = p.device
+            spans += self._span(p)
+        spans.sort()
+        for (_, end), (start, _) in zip(spans, spans[1:]):
+            if start < end:
+                raise ValueError("two parameters share memory, or one is given twice")
+        super().add_param_group(group)
+        self._number()
+
+    @staticmethod
+    def _span(p):
+        a = p.data_ptr()
+        return [(a, a + p.numel() * p.element_size())] if p.numel() else []
+
+    def _number(self):
+        self._first = []
+        n = 0
+        for g in self.param_groups:
+            self._first.append(n)
+            n += len(g["params"])
+        self._total = n
+
+    # ------------------------------------------------------------------- state
+    def _new_state(self, p, g):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the optimizer's state must be there before a step is captured: "
+                               "call init_state(), or take a step, first")
+        zeros = lambda n, dt: torch.zeros(n, dtype=torch.uint8, device=p.device).view(dt)  # noqa: E731
+        s = dict(step=torch.zeros((), dtype=torch.int64, device=p.device))
+        if g["state_bits"] == 8:
+            n = _reals(p)
+            s["exp_avg"] = zeros(n, torch.float8_e4m3fn)
+            s["exp_avg_sq"] = zeros(n, torch.float8_e5m2)
+            for k in ("exp_avg_scale", "exp_avg_sq_scale"):
+                s[k] = zeros(-(-n // BLOCK), torch.float8_e8m0fnu)
+                s[k].view(torch.uint8).fill_(1)
+        else:
+            dt = torch.complex64 if p.is_complex() else torch.float32
+            s["exp_avg"] = torch.zeros_like(p, dtype=dt, requires_grad=False)
+            s["exp_avg_sq"] = torch.zeros_like(p, dtype=dt, requires_grad=False)
+        if g["master"] and p.dtype in (torch.bfloat16, torch.float16):
+            s["master"] = p.detach().float()
+        return s
+
+    @staticmethod
+    def _check_state(s, p, g):
+        """a parameter's state as the kernels take it, or ValueError"""
+        eight = g["state_bits"] == 8
+        n = _reals(p)
+        want = {"exp_avg": torch.float8_e4m3fn, "exp_avg_sq": torch.float8_e5m2,
+                "exp_avg_scale": torch.float8_e8m0fnu,
+                "exp_avg_sq_scale": torch.float8_e8m0fnu} if eight else \
+               dict.fromkeys(("exp_avg", "exp_avg_sq"),
+                             torch.complex64 if p.is_complex() else torch.float32)
+        if g["master"] and p.dtype in (torch.bfloat16, torch.float16):
+            want["master"] = torch.float32
+        want["step"] = torch.int64
+        for k, dt in want.items():
+            t = s.get(k)
+            if not torch.is_tensor(t) or t.dtype != dt or t.device != p.device:
+                raise ValueError(f"state {k!r} must be a {dt} tensor on {p.device}")
+            if k == "step":
+                fits = t.numel() == 1
+            elif eight and k != "master":
+                fits = t.is_contiguous() and t.numel() == (
+                    -(-n // BLOCK) if k.endswith("scale") else n)
+            else:
+                fits = t.shape == p.shape and _dense(t) and _same_order(t, p)
+            if not fits:
+                raise ValueError(f"state {k!r} does not fit its parameter {tuple(p.shape)}")
+
+    @torch.no_grad()
+    def init_state(self):
+        """make what a step needs and is not there yet: the state of every
+        parameter (zero moments), the workspace"""
+        if self._dev is not None:
+            self._workspace(self._total)
+        for g in self.param_groups:
+            for p in g["params"]:
+                if not self.state.get(p):
+                    self.state[p] = self._new_state(p, g)
+
+    def load_state_dict(self, state_dict):
+        state_dict = dict(state_dict)
+        saved = state_dict["state"]
+        groups = state_dict["param_groups"]
+        # the base class would cast the state to the parameters' types: it
+        # only takes the groups, the state is laid out here
+        super().load_state_dict(dict(state_dict, state={}))
+        for g in self.param_groups:
+            for k, v in self.defaults.items():
+                g.setdefault(k, v)
+        new = {}
+        for old, g in zip(groups, self.param_groups):
+            for i, p in zip(old["params"], g["params"]):
+                if not saved.get(i):
+                    continue
+                s = {}
+                for k, v in saved[i].items():
+                    if k == "step":
+                        s[k] = torch.as_tensor(v).detach().to(p.device, torch.int64).reshape(()).clone()
+                    elif torch.is_tensor(v):
+                        v = v.detach().to(p.device, copy=True)
+                        if v.shape == p.shape and not _same_order(v, p):
+                            v = torch.empty_like(p, dtype=v.dtype, requires_grad=False).copy_(v)
+                        s[k] = v
+                if g["master"] and "master" not in s and p.dtype in (torch.bfloat16, torch.float16):
+                    s["master"] = p.detach().float()
+                self._check_state(s, p, g)
+                new[p] = s
+        self.state.clear()
+        self.state.update(new)
+
+    # -------------------------------------------------------------------- step
+    def _grad(self, p):
+        g = p.grad
+        if g.is_sparse or g.layout != torch.strided:
+            raise RuntimeError("sparse gradients are not supported")
+        if g.dtype != p.dtype or g.device != p.device or g.shape != p.shape:
+            raise ValueError(f"a gradient must be {p.dtype} {tuple(p.shape)} on {p.device}, got "
+                             f"{g.dtype} {tuple(g.shape)} on {g.device}")
+        if g.is_conj() or g.is_neg() or not _dense(g) or not _same_order(g, p):
+            g = torch.empty_like(p, requires_grad=False).copy_(g)
+        return g
+
+    def _workspace(self, count):
+        """grow-only; an outgrown one is kept: a captured graph may address it"""
+        need = _native.lib().cqt_adamw_workspace_bytes(count)
+        if self._ws is None or self._ws.numel() < need or (
+                self.max_norm is not None and self.grad_norm is None):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the optimizer's workspace must be there before a step is "
+                                   "captured: call init_state(), or take a step, first")
+            self._retired.append(self._ws)
+            self._ws = torch.zeros(need, dtype=torch.uint8, device=self._dev)
+            if self.max_norm is not None and self.grad_norm is None:
+                self.grad_norm = torch.zeros((), dtype=torch.float32, device=self._dev)
+        return self._ws
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        """one step of every parameter that has a gradient; returns what
+        ``closure`` (evaluated first, with gradients enabled) returns"""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        lists, keep = [], []
+        for g, first in zip(self.param_groups, self._first):
+            todo = []
+            for k, p in enumerate(g["params"]):
+                if p.grad is None or not p.numel():
+                    continue
+                s = self.state.get(p)
+                if not s:
+                    s = self.state[p] = self._new_state(p, g)
+                grad = self._grad(p)
+                keep.append(grad)
+                self._check_state(s, p, g)
+                at = lambda k: s[k].data_ptr() if k in s else None  # noqa: E731
+                todo.append(_native.CqtAdamwTensor(
+                    p.data_ptr(), grad.data_ptr(), at("master") if g["master"] else None,
+                    at("exp_avg"), at("exp_avg_sq"), at("exp_avg_scale"), at("exp_avg_sq_scale"),
+                    at("step"), _reals(p), _TYPES[p.dtype], first + k))
+            lists.append((_native.CqtAdamwTensor * len(todo))(*todo))
+        if self._dev is None:
+            return loss
+        with torch.cuda.device(self._dev):
+            self._launch(lists)
+        return loss
+
+    def _launch(self, lists):
+        L, stream = _native.lib(), _raw_stream_of(self._dev.index)
+        ws = self._workspace(self._total)
+        if self.max_norm is not None:
+            every = lists[0] if len(lists) == 1 else (
+                (_native.CqtAdamwTensor * sum(map(len, lists)))(*(t for x in lists for t in x)))
+            _native._check(L.cqt_grad_norm(every, len(every), self.grad_norm.data_ptr(),
+                                           ws.data_ptr(), ws.numel(), stream), "cqt_grad_norm")
+        for g, todo in zip(self.param_groups, lists):
+            if not len(todo):
+                continue
+            lr = g["lr"]
+            on_device = torch.is_tensor(lr) and lr.device == self._dev
+            args = _native.CqtAdamwArgs(
+                0.0 if on_device else float(lr), *map(float, g["betas"]), float(g["eps"]),
+                float(g["weight_decay"]), self.max_norm or 0.0,
+                lr.data_ptr() if on_device else None, int(self.max_norm is not None), self.seed)
+            _native._check(L.cqt_adamw_step(todo, len(todo), g["state_bits"], ctypes.byref(args),
+                                            ws.data_ptr(), ws.numel(), stream), "cqt_adamw_step")

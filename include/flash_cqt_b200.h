@@ -308,6 +308,101 @@ const char* cqt_last_error(void);
 /* ABI version of this header (major * 100 + minor). */
 int cqt_version(void);
 
+/* ---- AdamW over many tensors --------------------------------------------
+ *
+ * One step of every tensor of a list, in place; t is the tensor's own count:
+ *   g' = g c,  c = min(1, max_norm / (norm + 1e-6)) with use_norm, else 1
+ *   m  = b1 m + (1 - b1) g';   v = b2 v + (1 - b2) g'^2;   t = t + 1
+ *   p  = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * computed in 32 bits; a 16-bit parameter is rounded once.  Arrays of a tensor
+ * lie in one order (element i of each belongs to element i of the others).
+ * state_bits 32: exp_avg and exp_avg_sq are float32.  state_bits 8: exp_avg
+ * holds e4m3 codes and exp_avg_sq e5m2 codes; 256 consecutive elements share
+ * a scale 2^(byte - 127) of each, rounded stochastically by a hash of (seed,
+ * t, ordinal, element).  No two arrays that are written may overlap. */
+#define CQT_F32 0
+#define CQT_BF16 1
+#define CQT_F16 2
+
+typedef struct cqt_adamw_tensor {
+    void* param;                /* numel values of `dtype` */
+    const void* grad;           /* numel values of `dtype` */
+    float* master;              /* 32-bit copy of a 16-bit parameter, or NULL */
+    void* exp_avg;
+    void* exp_avg_sq;
+    uint8_t* exp_avg_scale;     /* state_bits 8: [ceil(numel / 256)] */
+    uint8_t* exp_avg_sq_scale;
+    int64_t* step;              /* device: steps taken so far */
+    int64_t numel;              /* 0: the tensor is left out */
+    int32_t dtype;              /* CQT_F32, CQT_BF16, CQT_F16 */
+    int32_t ordinal;            /* the tensor's number in the rounding hash */
+} cqt_adamw_tensor;
+
+typedef struct cqt_adamw_args {
+    double lr, beta1, beta2, eps, weight_decay;
+    double max_norm;            /* with use_norm */
+    const float* lr_dev;        /* not NULL: the rate is read from the device */
+    int32_t use_norm;           /* scale by the norm that cqt_grad_norm left in
+                                   the workspace */
+    uint32_t seed;
+} cqt_adamw_args;
+
+/* Workspace of the two calls below (16-byte aligned, zeroed once when it is
+ * allocated, for one stream at a time). */
+size_t cqt_adamw_workspace_bytes(int count);
+/* sqrt of the sum of the squares of all gradients (grad, numel and dtype of
+ * each entry are used), summed in 64 bits in a fixed order; kept in the
+ * workspace and, if norm is not NULL, stored there as float32. */
+int cqt_grad_norm(const cqt_adamw_tensor* tensors, int count, float* norm,
+                  void* workspace, size_t workspace_bytes, void* stream);
+int cqt_adamw_step(const cqt_adamw_tensor* tensors, int count, int state_bits,
+                   const cqt_adamw_args* args, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/* ---- coefficient cache ---------------------------------------------------
+ *
+ * The newest `capacity` slices of `rows` streams in 8 bits.  Slice k of a
+ * stream lies in slot k mod capacity.  16 consecutive coefficients of the
+ * heap share a scale 2^(byte - 127), the least that brings their largest
+ * finite magnitude to 127 (int8) or 448 (e4m3) or below.  A code is the value
+ * over the scale, rounded to nearest even; -128 (int8) or NaN (e4m3) stands
+ * for a value that is not finite. */
+#define CQT_CACHE_INT8 0
+#define CQT_CACHE_E4M3 1
+
+typedef struct cqt_cache {
+    void* codes;                /* [rows][capacity][ncoef][2], 16-byte aligned */
+    uint8_t* scales;            /* [rows][capacity][ncoef / 16] */
+    int64_t* length;            /* device [rows]: slices written so far */
+    void* workspace;            /* 256 bytes, zeroed once */
+    int32_t rows, capacity;
+    int32_t format;             /* CQT_CACHE_INT8 or CQT_CACHE_E4M3 */
+    int32_t ngroups;            /* <= 16 */
+    const int32_t* group_count; /* host: bands of each group */
+    const int32_t* group_len;   /* host: block length, a power of two >= 16 */
+} cqt_cache;
+
+/* One group's coefficients: value (row, slice, band, t) lies at
+ * data + row * row_stride + slice * slice_stride + band * band_stride + t,
+ * counted in complex values. */
+typedef struct cqt_cache_part {
+    void* data;
+    int64_t row_stride, slice_stride, band_stride;
+} cqt_cache_part;
+
+/* Write the first counts[row] (device, or NULL: all) of `slices` slices of
+ * every stream behind its last one and advance its length.  parts: complex64,
+ * 8-byte aligned, one entry per group.  Slots of other slices stay as they
+ * are. */
+int cqt_cache_append(const cqt_cache* cache, const cqt_cache_part* parts, int slices,
+                     const int64_t* counts, void* stream);
+/* Read slices [end - slices, end) of every stream, end = ends[row] (device) or
+ * the stream's length; slices that are not in the ring read as zeros.  parts:
+ * pairs of `dtype` (CQT_F32 is complex64), 16-byte aligned, strides a multiple
+ * of 16 bytes. */
+int cqt_cache_window(const cqt_cache* cache, const cqt_cache_part* parts, int slices,
+                     const int64_t* ends, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,124 @@
+"""CPU checks of AdamW: refusals, the C entries' argument checks, the rounding
+noise of the 8-bit moments."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import plain_optim as po
+from flash_cqt_b200 import AdamW, _native
+
+
+def leaf(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype, requires_grad=True)
+
+
+@pytest.mark.parametrize("kw, what", [
+    (dict(lr=-1.0), "lr"), (dict(lr=float("nan")), "lr"), (dict(betas=(1.0, 0.9)), "betas"),
+    (dict(betas=(0.9, -0.1)), "betas"), (dict(eps=-1e-8), "eps"), (dict(weight_decay=-1.0), "eps"),
+    (dict(state_bits=16), "state_bits"), (dict(max_norm=0.0), "max_norm"),
+    (dict(max_norm=float("nan")), "max_norm"), (dict(lr=torch.ones(2)), "lr")])
+def test_bad_options(kw, what):
+    with pytest.raises(ValueError, match=what):
+        AdamW([leaf(3)], **kw)
+
+
+def test_bad_parameters():
+    with pytest.raises(TypeError, match="float32"):
+        AdamW([leaf(3, dtype=torch.float64)])
+    with pytest.raises(TypeError, match="float32"):
+        AdamW([leaf(3, dtype=torch.complex128)])
+    with pytest.raises(ValueError, match="dense"):
+        AdamW([torch.zeros(4, 6)[:, ::2].requires_grad_()])
+    with pytest.raises(ValueError, match="dense"):
+        AdamW([torch.zeros(1, 4).expand(3, 4).requires_grad_()])
+    with pytest.raises(RuntimeError, match="CUDA devices only"):
+        AdamW([leaf(3)])
+    with pytest.raises(ValueError):
+        AdamW([])
+
+
+def test_dense_orders():
+    from flash_cqt_b200.optim import _dense, _same_order
+    a = torch.zeros(2, 3, 4, 5)
+    assert _dense(a) and _dense(a.permute(2, 0, 3, 1)) and _dense(torch.zeros(()))
+    assert _dense(a.to(memory_format=torch.channels_last))
+    assert not _dense(a[:, 1:]) and not _dense(a[..., ::2])
+    assert _dense(torch.zeros(3, 1)[:, :1]) and _dense(torch.zeros(0, 4))
+    assert not _same_order(torch.zeros(3, 4), torch.zeros(4, 3).t())
+    assert _same_order(torch.zeros(1, 4), torch.zeros(4, 1).t())
+
+
+def test_c_entries_refuse():
+    L = _native.lib()
+    T = _native.CqtAdamwTensor
+    ws = ctypes.create_string_buffer(1 << 16)
+    at = (ctypes.addressof(ws) + 15) & ~15
+    need = L.cqt_adamw_workspace_bytes(1)
+    assert need < 1 << 15 and L.cqt_adamw_workspace_bytes(-1) == 0
+    assert L.cqt_adamw_workspace_bytes(361) > need
+    good = _native.CqtAdamwArgs(1e-3, 0.9, 0.999, 1e-8, 0.0, 0.0, None, 0, 0)
+
+    def step(t, args=good, bits=32, count=1, w=at, size=need):
+        rc = L.cqt_adamw_step(ctypes.byref(t) if t is not None else None, count, bits,
+                              ctypes.byref(args), w, size, None)
+        return rc, L.cqt_last_error().decode()
+
+    # addresses that are never read: every call is refused on the host
+    ok = dict(param=64, grad=64, exp_avg=64, exp_avg_sq=64, step=64, numel=4)
+    assert step(T(**ok), w=None) == (-1, "workspace missing or smaller than cqt_adamw_workspace_bytes")
+    assert step(T(**ok), size=need - 1)[0] == -1
+    assert step(T(**ok), w=at + 4)[1] == "workspace not 16-byte aligned"
+    assert step(T(**ok), count=-1)[1] == "negative tensor count"
+    assert step(None)[1] == "null tensors or arguments"
+    assert step(T(**ok), bits=16)[1] == "state_bits must be 8 or 32"
+    for bad in (dict(grad=None), dict(grad=66), dict(param=None), dict(param=65), dict(exp_avg=None),
+                dict(exp_avg_sq=None), dict(exp_avg_sq=66), dict(step=None), dict(step=68),
+                dict(master=64), dict(numel=-1), dict(dtype=3), dict(numel=1 << 43)):
+        rc, msg = step(T(**{**ok, **bad}))
+        assert rc == -1 and msg, bad
+    assert step(T(**ok), bits=8)[1] == "null scales or misaligned moments"
+    for k, v in (("beta1", 1.0), ("beta2", -0.1), ("beta1", float("nan")), ("eps", -1.0)):
+        a = _native.CqtAdamwArgs(1e-3, 0.9, 0.999, 1e-8, 0.0, 0.0, None, 0, 0)
+        setattr(a, k, v)
+        assert "betas" in step(T(**ok), a)[1]
+    a = _native.CqtAdamwArgs(1e-3, 0.9, 0.999, 1e-8, 0.0, 0.0, None, 1, 0)
+    assert step(T(**ok), a)[1] == "max_norm must be positive"
+    assert L.cqt_grad_norm(ctypes.byref(T(numel=3)), 1, None, at, need, None) == -1
+    assert L.cqt_grad_norm(None, 1, None, at, need, None) == -1
+    # a list without elements is no work
+    assert step(T(numel=0))[0] == 0 and step(None, count=0)[0] == 0
+
+
+def test_noise_is_uniform_and_independent():
+    n = 1 << 16
+    h = po.noise(7, 3, 2, n)
+    for bits in (h & np.uint32(0xffff), h >> np.uint32(16)):
+        # 64 classes of 1024 expected: chi square of 63 degrees of freedom is
+        # below 63 + 6 sqrt(126) = 130 but for one in a million
+        c = np.bincount(bits >> np.uint32(10), minlength=64)
+        assert ((c - 1024.0) ** 2 / 1024).sum() < 130
+    # neighbours, steps, tensors and seeds: correlations of n pairs are below
+    # 6 / sqrt(n)
+    f = lambda x: (x & np.uint32(0xffff)) / 65536.0 - 0.5  # noqa: E731
+    a = f(h)
+    for b in (f(h >> np.uint32(16)), np.roll(a, 1), f(po.noise(7, 4, 2, n)), f(po.noise(7, 3, 3, n)),
+              f(po.noise(8, 3, 2, n))):
+        assert abs((a * b).mean() * 12) < 6 / np.sqrt(n)
+
+
+def test_rounding_is_unbiased():
+    """the mean over many draws is the value itself (within 6 deviations)"""
+    n = 1 << 15
+    for x in (0.3, 1.0, 447.0, 2.0 ** -5):
+        v = np.full(n, x)
+        v[::po.BLOCK] = 448.0
+        s = po.scales(v, 448.0)
+        r = po.round_m(v, s, po.noise(1, 1, 0, n))[v == x]
+        step = 2.0 ** (np.floor(np.log2(x)) - 3)
+        assert abs(r.mean() - x) < 6 * step / 2 / np.sqrt(r.size) + step * 2.0 ** -17
+    v = np.full(n, 3.3)
+    v[::po.BLOCK] = 57344.0
+    r = po.round_v(v, po.scales(v, 57344.0), po.noise(1, 1, 0, n))[v == 3.3]
+    assert abs(r.mean() - 3.3) < 6 * 0.25 / np.sqrt(r.size)
