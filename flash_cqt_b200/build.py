@@ -90,7 +90,8 @@ def build_torch_ops(force=False, verbose=False):
     from torch.utils import cpp_extension as ce
     out = torch_ops_path()
     out.parent.mkdir(parents=True, exist_ok=True)
-    if not force and out.exists() and out.stat().st_mtime >= TORCH_OPS_SRC.stat().st_mtime:
+    newest = max(p.stat().st_mtime for p in [TORCH_OPS_SRC, *INCLUDE.glob("*.h")])
+    if not force and out.exists() and out.stat().st_mtime >= newest:
         return out
     inc = ce.include_paths(device_type="cuda") + [sysconfig.get_paths()["include"]]
     libdirs = ce.library_paths(device_type="cuda")
@@ -101,7 +102,7 @@ def build_torch_ops(force=False, verbose=False):
     cmd = [cxx, "-O3", "-std=c++17", "-fPIC", "-shared",
            "-DTORCH_EXTENSION_NAME=_torchops", "-DTORCH_API_INCLUDE_EXTENSION_H",
            f"-D_GLIBCXX_USE_CXX11_ABI={abi}",   # default visibility: c10 exception types must match
-           *[f"-I{d}" for d in inc], str(TORCH_OPS_SRC), "-o", str(out),
+           f"-I{INCLUDE}", *[f"-I{d}" for d in inc], str(TORCH_OPS_SRC), "-o", str(out),
            *[f"-L{d}" for d in libdirs], *[f"-Wl,-rpath,{d}" for d in libdirs[:1]],
            "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
     if verbose:

@@ -86,6 +86,13 @@ class CoefCache:
             self._ws.data_ptr(), self.rows, self.capacity, self._format, len(self.gspec),
             ctypes.cast(self._bands, _native._i32p), ctypes.cast(self._lens, _native._i32p))
 
+        mod = _native.torch_ops()   # the same calls from C++ (None: ctypes)
+        self._h = None if mod is None else mod.CacheHandle(
+            *[_native.fn_address(n) for n in ("cqt_cache_append", "cqt_cache_window",
+                                              "cqt_last_error")],
+            self.codes, self.scales, self.length, self._ws, self.capacity, self._format,
+            [b for b, _ in self.gspec], [M for _, M in self.gspec], self.ngroups)
+
     def nbytes(self):
         """bytes of the store"""
         return self.codes.numel() + self.scales.numel()
@@ -127,14 +134,16 @@ class CoefCache:
         return t.contiguous()
 
     # ------------------------------------------------------------------- calls
-    @torch.no_grad()
     def append(self, blocks, side, counts=None):
         """the slices of (blocks, side) -- blocks [*lead, b, S * M], side
         [*lead, S, 1, M], as ``SlicedCQT.fwd`` returns them, or one slice with
         side [*lead, 1, M] -- behind those that the streams have.  counts (int64
         [*lead] on the device): how many of the S slices each stream has
         (padded batches); the others are left out."""
-        blocks, side, S = self._slices(blocks, side)
+        if self._h is not None and side is not None and \
+                self._h.append([*blocks, *side], counts):
+            return
+        blocks, side, S = self._slices(blocks, side)   # refuses what does not fit
         counts = self._numbers(counts, "counts")
         parts = (_native.CqtCachePart * len(self.gspec))()
         keep = []
@@ -153,7 +162,6 @@ class CoefCache:
                 ctypes.byref(self._desc), parts, S, counts.data_ptr() if counts is not None else None,
                 _raw_stream_of(self.dev.index)), "cqt_cache_append")
 
-    @torch.no_grad()
     def window(self, n, dtype=torch.complex64, end=None):
         """slices [end - n, end) of every stream as (blocks, side) in the layout
         of ``SlicedCQT.fwd``: blocks [*lead, b, n * M], side [*lead, n, 1, M].
@@ -167,6 +175,8 @@ class CoefCache:
         if dtype not in _OUT:
             raise TypeError("dtype must be complex64, float32, bfloat16 or float16, "
                             f"got {dtype}")
+        if self._h is not None:
+            return self._h.window(n, dtype, _OUT[dtype], end)
         end = self._numbers(end, "end")
         cplx = dtype == torch.complex64
         tail = () if cplx else (2,)

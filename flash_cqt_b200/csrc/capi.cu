@@ -1037,6 +1037,7 @@ int cqt_adamw_step(const cqt_adamw_tensor* tensors, int count, int state_bits,
         return fail(CQT_ERR_ARG, "state_bits must be 8 or 32");
     if (!(a->beta1 >= 0 && a->beta1 < 1 && a->beta2 >= 0 && a->beta2 < 1) || !(a->eps >= 0))
         return fail(CQT_ERR_ARG, "betas must lie in [0, 1) and eps must not be negative");
+    if (!a->lr_dev && !(a->lr >= 0)) return fail(CQT_ERR_ARG, "lr must not be negative");
     if (a->use_norm && !(a->max_norm > 0)) return fail(CQT_ERR_ARG, "max_norm must be positive");
     OptArgs o{};
     o.lr = a->lr;

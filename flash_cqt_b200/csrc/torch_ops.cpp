@@ -10,7 +10,13 @@
 // forward returns per-group complex views, the backward of the analysis is
 // the transpose of the analysis, that of the synthesis the transpose of the
 // synthesis, nothing saved for backward).
+//
+// Also the per-call host work of AdamW.step (gradients, addresses and checks of
+// every parameter) and of CoefCache.append / window, which have no counterpart
+// there.
 #include <torch/extension.h>
+
+#include "flash_cqt_b200.h"
 
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -460,6 +466,399 @@ struct Handle {
     }
 };
 
+// ---------------------------------------------------------------------------
+// AdamW: one step's host work
+using FnGradNorm = decltype(&cqt_grad_norm);
+using FnAdamw = decltype(&cqt_adamw_step);
+
+// whether the elements fill one stretch of memory and element i of a's is
+// element i of b's (sizes are equal)
+bool same_order(const at::Tensor& a, const at::Tensor& b) {
+    for (int64_t d = 0; d < a.dim(); ++d)
+        if (a.size(d) != 1 && a.stride(d) != b.stride(d)) return false;
+    return true;
+}
+
+// The parameters of an optimizer with the states that it holds for them.  It
+// remembers the Python objects that it was built from -- the lists of
+// parameters, the state dictionary, every parameter's own dictionary and what
+// is in them -- and refuses to step (the caller then builds another) when any of
+// them has been replaced.
+struct AdamWPlan {
+    struct Slot {
+        at::Tensor p;
+        at::Tensor m, v, ms, vs, step, master;   // undefined: no state yet
+        cqt_adamw_tensor d{};
+    };
+    struct Group {
+        std::vector<Slot> slots;
+        std::vector<PyObject*> params;   // the list's items (kept alive by `held`)
+        int bits = 32;
+        bool master = false;
+    };
+    std::vector<Group> groups;
+    std::vector<PyObject*> seen;         // keys and values of the state, in order
+    std::vector<pybind11::object> held;
+    c10::DeviceIndex device;
+    FnGradNorm norm_fn;
+    FnAdamw step_fn;
+    FnLastError last_error;
+    std::vector<cqt_adamw_tensor> todo;
+    std::vector<int64_t> ends;           // of each group in todo
+    std::vector<at::Tensor> keep;
+
+    static void walk(PyObject* state, std::vector<PyObject*>& out) {
+        PyObject *k, *v;
+        Py_ssize_t at = 0;
+        while (PyDict_Next(state, &at, &k, &v)) {
+            out.push_back(k);
+            out.push_back(v);
+            if (!PyDict_Check(v)) continue;
+            PyObject *kk, *vv;
+            Py_ssize_t inner = 0;
+            while (PyDict_Next(v, &inner, &kk, &vv)) out.push_back(vv);
+        }
+    }
+
+    AdamWPlan(int device_, uintptr_t norm, uintptr_t step, uintptr_t error,
+              pybind11::list param_groups, pybind11::dict state)
+        : device((c10::DeviceIndex)device_), norm_fn(reinterpret_cast<FnGradNorm>(norm)),
+          step_fn(reinterpret_cast<FnAdamw>(step)),
+          last_error(reinterpret_cast<FnLastError>(error)) {
+        int32_t ordinal = 0;
+        for (auto g : param_groups) {
+            pybind11::dict group = g.cast<pybind11::dict>();
+            groups.emplace_back();
+            Group& out = groups.back();
+            out.bits = group["state_bits"].cast<int>();
+            out.master = group["master"].cast<bool>();
+            pybind11::list params = group["params"].cast<pybind11::list>();
+            for (auto p : params) {
+                held.push_back(pybind11::reinterpret_borrow<pybind11::object>(p));
+                out.params.push_back(p.ptr());
+                out.slots.emplace_back();
+                Slot& s = out.slots.back();
+                s.p = p.cast<at::Tensor>();
+                s.d.ordinal = ordinal++;
+                s.d.numel = s.p.numel() * (s.p.is_complex() ? 2 : 1);
+                s.d.dtype = s.p.scalar_type() == at::kBFloat16 ? CQT_BF16
+                            : s.p.scalar_type() == at::kHalf   ? CQT_F16 : CQT_F32;
+                pybind11::object mine = pybind11::none();
+                if (state.contains(p)) mine = state[p];
+                if (!pybind11::isinstance<pybind11::dict>(mine)) continue;
+                pybind11::dict d = mine.cast<pybind11::dict>();
+                auto get = [&](const char* k) {
+                    return d.contains(k) ? d[k].cast<at::Tensor>() : at::Tensor();
+                };
+                s.m = get("exp_avg");
+                s.v = get("exp_avg_sq");
+                s.step = get("step");
+                if (out.bits == 8) {
+                    s.ms = get("exp_avg_scale");
+                    s.vs = get("exp_avg_sq_scale");
+                }
+                if (out.master && s.d.dtype != CQT_F32) s.master = get("master");
+            }
+        }
+        walk(state.ptr(), seen);
+        for (PyObject* o : seen) held.push_back(pybind11::reinterpret_borrow<pybind11::object>(o));
+    }
+
+    // whether what this was built from is still what the optimizer holds
+    bool current(const pybind11::list& param_groups, const pybind11::dict& state) const {
+        if (param_groups.size() != groups.size()) return false;
+        PyObject *k, *v;
+        Py_ssize_t at = 0;
+        size_t i = 0;
+        auto next = [&](PyObject* o) { return i < seen.size() && seen[i++] == o; };
+        while (PyDict_Next(state.ptr(), &at, &k, &v)) {
+            if (!next(k) || !next(v)) return false;
+            if (!PyDict_Check(v)) continue;
+            PyObject *kk, *vv;
+            Py_ssize_t inner = 0;
+            while (PyDict_Next(v, &inner, &kk, &vv))
+                if (!next(vv)) return false;
+        }
+        return i == seen.size();
+    }
+
+    // fills `todo` with the parameters that have gradients; false where one of
+    // them has no state yet, or not one for its present shape
+    bool gather(const pybind11::list& param_groups) {
+        todo.clear();
+        ends.clear();
+        keep.clear();
+        size_t k = 0;
+        for (auto gr : param_groups) {
+            Group& g = groups[k++];
+            PyObject* group = gr.ptr();
+            PyObject* params = PyDict_GetItemString(group, "params");
+            if (!params || !PyList_Check(params) ||
+                (size_t)PyList_GET_SIZE(params) != g.params.size() ||
+                number(item(group, "state_bits")) != g.bits ||
+                PyObject_IsTrue(item(group, "master")) != (g.master ? 1 : 0))
+                return false;
+            for (size_t i = 0; i < g.slots.size(); ++i) {
+                if (PyList_GET_ITEM(params, (Py_ssize_t)i) != g.params[i]) return false;
+                Slot& s = g.slots[i];
+                const at::Tensor& p = s.p;
+                const at::Tensor& grad = p.grad();
+                if (!grad.defined() || p.numel() == 0) continue;
+                if (!s.m.defined() || !s.v.defined() || !s.step.defined()) return false;
+                TORCH_CHECK(grad.layout() == at::kStrided, "sparse gradients are not supported");
+                TORCH_CHECK_VALUE(grad.scalar_type() == p.scalar_type() &&
+                                      grad.device() == p.device() && grad.sizes() == p.sizes(),
+                                  "a gradient must be ", p.scalar_type(), " ", p.sizes(), " on ",
+                                  p.device(), ", got ", grad.scalar_type(), " ", grad.sizes(),
+                                  " on ", grad.device());
+                // the parameter's storage may have been exchanged
+                const int64_t n = p.numel() * (p.is_complex() ? 2 : 1);
+                if (n != s.d.numel || !p.is_non_overlapping_and_dense() || p.get_device() != device)
+                    return false;
+                if (g.bits == 32 && (s.m.sizes() != p.sizes() || !same_order(s.m, p) ||
+                                     s.v.sizes() != p.sizes() || !same_order(s.v, p)))
+                    return false;
+                at::Tensor use = grad;
+                if (grad.is_conj() || grad.is_neg() || !same_order(grad, p)) {
+                    use = at::empty_like(p).copy_(grad);
+                    keep.push_back(use);
+                }
+                s.d.param = p.data_ptr();
+                s.d.grad = use.data_ptr();
+                s.d.master = s.master.defined() ? s.master.data_ptr<float>() : nullptr;
+                s.d.exp_avg = s.m.data_ptr();
+                s.d.exp_avg_sq = s.v.data_ptr();
+                s.d.exp_avg_scale =
+                    s.ms.defined() ? static_cast<uint8_t*>(s.ms.data_ptr()) : nullptr;
+                s.d.exp_avg_sq_scale =
+                    s.vs.defined() ? static_cast<uint8_t*>(s.vs.data_ptr()) : nullptr;
+                s.d.step = s.step.data_ptr<int64_t>();
+                todo.push_back(s.d);
+            }
+            ends.push_back((int64_t)todo.size());
+        }
+        return true;
+    }
+
+    // an option of a parameter group
+    static PyObject* item(PyObject* group, const char* key) {
+        PyObject* o = PyDict_GetItemString(group, key);
+        if (!o) throw pybind11::key_error(key);
+        return o;
+    }
+    static double number(PyObject* o) {
+        const double x = PyFloat_AsDouble(o);
+        if (x == -1.0 && PyErr_Occurred()) throw pybind11::error_already_set();
+        return x;
+    }
+
+    // one step; false (nothing done) when the plan does not fit any more
+    bool step(pybind11::list param_groups, pybind11::dict state, pybind11::object max_norm,
+              uint32_t seed, const at::Tensor& ws, const c10::optional<at::Tensor>& norm) {
+        at::NoGradGuard no_grad;
+        if (!current(param_groups, state)) return false;
+        Ops::DeviceSwitch sw(device);
+        if (!gather(param_groups)) return false;
+        void* stream = at::cuda::getCurrentCUDAStream(device).stream();
+        auto check = [&](int rc, const char* what) {
+            TORCH_CHECK(rc == 0, what, " failed (", rc, "): ", last_error());
+        };
+        cqt_adamw_args a{};
+        a.use_norm = max_norm.is_none() ? 0 : 1;
+        a.max_norm = a.use_norm ? number(max_norm.ptr()) : 0.0;
+        a.seed = seed;
+        if (a.use_norm)
+            check(norm_fn(todo.data(), (int)todo.size(), norm->data_ptr<float>(), ws.data_ptr(),
+                          (size_t)ws.numel(), stream),
+                  "cqt_grad_norm");
+        int64_t first = 0;
+        size_t k = 0;
+        for (auto gr : param_groups) {
+            const int64_t last = ends[k];
+            const int bits = groups[k++].bits;
+            if (last == first) continue;
+            PyObject* g = gr.ptr();
+            PyObject* lr = item(g, "lr");
+            PyObject* betas = item(g, "betas");
+            if (THPVariable_Check(lr)) {
+                const at::Tensor& t = THPVariable_Unpack(lr);
+                if (t.is_cuda()) {
+                    TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat, "a device lr must be float32, got ",
+                                     t.scalar_type());
+                    TORCH_CHECK_VALUE(t.numel() == 1 && t.get_device() == device,
+                                      "a device lr must hold one number on cuda:", (int)device);
+                    a.lr_dev = t.data_ptr<float>();
+                    a.lr = 0;
+                } else {
+                    a.lr_dev = nullptr;
+                    a.lr = t.item<double>();
+                }
+            } else {
+                a.lr_dev = nullptr;
+                a.lr = number(lr);
+            }
+            pybind11::sequence bs = pybind11::reinterpret_borrow<pybind11::sequence>(betas);
+            a.beta1 = bs[0].cast<double>();
+            a.beta2 = bs[1].cast<double>();
+            a.eps = number(item(g, "eps"));
+            a.weight_decay = number(item(g, "weight_decay"));
+            check(step_fn(todo.data() + first, (int)(last - first), bits, &a, ws.data_ptr(),
+                          (size_t)ws.numel(), stream),
+                  "cqt_adamw_step");
+            first = last;
+        }
+        keep.clear();
+        return true;
+    }
+};
+
+// ---------------------------------------------------------------------------
+// CoefCache: the per-call host work of append and window
+using FnCacheAppend = decltype(&cqt_cache_append);
+using FnCacheWindow = decltype(&cqt_cache_window);
+
+struct CacheHandle {
+    at::Tensor codes, scales, length, ws;
+    std::vector<int64_t> lead;
+    std::vector<int32_t> bands, lens;
+    int64_t ngroups, rows = 1, ncoef = 0;
+    c10::DeviceIndex device;
+    cqt_cache desc{};
+    FnCacheAppend append_fn;
+    FnCacheWindow window_fn;
+    FnLastError last_error;
+
+    CacheHandle(uintptr_t append, uintptr_t window, uintptr_t error, at::Tensor codes_,
+                at::Tensor scales_, at::Tensor length_, at::Tensor ws_, int64_t capacity,
+                int format, std::vector<int32_t> bands_, std::vector<int32_t> lens_,
+                int64_t ngroups_)
+        : codes(std::move(codes_)), scales(std::move(scales_)), length(std::move(length_)),
+          ws(std::move(ws_)), lead(length.sizes().vec()), bands(std::move(bands_)),
+          lens(std::move(lens_)), ngroups(ngroups_), device((c10::DeviceIndex)codes.get_device()),
+          append_fn(reinterpret_cast<FnCacheAppend>(append)),
+          window_fn(reinterpret_cast<FnCacheWindow>(window)),
+          last_error(reinterpret_cast<FnLastError>(error)) {
+        for (int64_t d : lead) rows *= d;
+        for (size_t k = 0; k < bands.size(); ++k) ncoef += (int64_t)bands[k] * lens[k];
+        desc.codes = codes.data_ptr();
+        desc.scales = static_cast<uint8_t*>(scales.data_ptr());
+        desc.length = length.data_ptr<int64_t>();
+        desc.workspace = ws.data_ptr();
+        desc.rows = (int32_t)rows;
+        desc.capacity = (int32_t)capacity;
+        desc.format = format;
+        desc.ngroups = (int32_t)bands.size();
+        desc.group_count = bands.data();
+        desc.group_len = lens.data();
+    }
+    CacheHandle(const CacheHandle&) = delete;   // desc points into the vectors
+
+    void check(int rc, const char* what) const {
+        TORCH_CHECK(rc == 0, what, " failed (", rc, "): ", last_error());
+    }
+
+    const int64_t* numbers(const c10::optional<at::Tensor>& t, const char* name,
+                           at::Tensor& hold) const {
+        if (!t) return nullptr;
+        TORCH_CHECK_VALUE(t->is_cuda() && t->get_device() == device &&
+                              t->scalar_type() == at::kLong && t->sizes() == at::IntArrayRef(lead),
+                          name, " must be an int64 tensor ", at::IntArrayRef(lead), " on cuda:",
+                          (int)device);
+        hold = t->contiguous();
+        return hold.data_ptr<int64_t>();
+    }
+
+    // false (nothing done) for shapes that the caller has to sort out or refuse
+    bool append(const std::vector<at::Tensor>& all, const c10::optional<at::Tensor>& counts) {
+        at::NoGradGuard no_grad;
+        const size_t L = lead.size();
+        if (all.size() != bands.size() || all[0].dim() != (int64_t)L + 2) return false;
+        const int64_t S = all[0].size((int64_t)L + 1) / lens[0];
+        cqt_cache_part parts[16];
+        for (size_t k = 0; k < all.size(); ++k) {
+            const at::Tensor& c = all[k];
+            if (!c.defined() || !c.is_cuda() || c.get_device() != device ||
+                c.scalar_type() != at::kComplexFloat || c.is_conj())
+                return false;
+            const bool side = (int64_t)k >= ngroups;
+            const int64_t b = bands[k], M = lens[k];
+            const int64_t want = !side || c.dim() == (int64_t)L + 2 ? (int64_t)L + 2 : (int64_t)L + 3;
+            if (c.dim() != want || c.sizes().slice(0, L) != at::IntArrayRef(lead)) return false;
+            const bool one = side && want == (int64_t)L + 2;
+            if (!side ? (c.size(L) != b || c.size(L + 1) != S * M)
+                      : one ? (S != 1 || c.size(L) != b || c.size(L + 1) != M)
+                            : (c.size(L) != S || c.size(L + 1) != b || c.size(L + 2) != M))
+                return false;
+            // the leading dimensions have to be one stride
+            if (c.stride(-1) != 1 || reinterpret_cast<uintptr_t>(c.data_ptr()) % 8) return false;
+            int64_t row = 0, span = 1;
+            for (size_t d = L; d-- > 0;) {
+                if (lead[d] == 1) continue;
+                if (span == 1) row = c.stride((int64_t)d);
+                else if (c.stride((int64_t)d) != row * span) return false;
+                span *= lead[d];
+            }
+            parts[k].data = c.data_ptr();
+            parts[k].row_stride = row;
+            if (!side) {
+                parts[k].slice_stride = M;
+                parts[k].band_stride = c.stride((int64_t)L);
+            } else {
+                parts[k].slice_stride = one ? 0 : c.stride((int64_t)L);
+                parts[k].band_stride = c.stride(one ? (int64_t)L : (int64_t)L + 1);
+            }
+        }
+        at::Tensor hold;
+        const int64_t* n = numbers(counts, "counts", hold);
+        Ops::DeviceSwitch sw(device);
+        check(append_fn(&desc, parts, (int)S, n, at::cuda::getCurrentCUDAStream(device).stream()),
+              "cqt_cache_append");
+        return true;
+    }
+
+    pybind11::tuple window(int64_t n, at::ScalarType dtype, int type,
+                           const c10::optional<at::Tensor>& end) {
+        at::NoGradGuard no_grad;
+        at::Tensor hold;
+        const int64_t* e = numbers(end, "end", hold);
+        const bool cplx = dtype == at::kComplexFloat;
+        const int64_t item = cplx ? 1 : 2;   // scalars of one coefficient
+        Ops::DeviceSwitch sw(device);
+        at::Tensor out = at::empty({rows * n * ncoef * item}, codes.options().dtype(dtype));
+        char* base = static_cast<char*>(out.data_ptr());
+        cqt_cache_part parts[16];
+        pybind11::list blocks, side;
+        int64_t off = 0;
+        for (size_t k = 0; k < bands.size(); ++k) {
+            const int64_t b = bands[k], M = lens[k], row = n * b * M;
+            parts[k] = {base + (size_t)off * item * out.element_size(), row, M, n * M};
+            std::vector<int64_t> sz(lead);
+            if ((int64_t)k < ngroups) {
+                sz.insert(sz.end(), {b, n * M});
+            } else {
+                parts[k].slice_stride = b * M;
+                parts[k].band_stride = M;
+                sz.insert(sz.end(), {n, b, M});
+            }
+            if (!cplx) sz.push_back(2);
+            std::vector<int64_t> st(sz.size());
+            int64_t step = 1;
+            for (size_t d = sz.size(); d-- > 0;) {
+                st[d] = step;
+                step *= sz[d] > 1 ? sz[d] : 1;
+            }
+            at::Tensor v = out.as_strided(sz, st, off * item);
+            if ((int64_t)k < ngroups) blocks.append(v);
+            else side.append(v);
+            off += rows * row;
+        }
+        check(window_fn(&desc, parts, (int)n, e, type,
+                        at::cuda::getCurrentCUDAStream(device).stream()),
+              "cqt_cache_window");
+        return pybind11::make_tuple(blocks, side);
+    }
+};
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -482,4 +881,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         .def("mse_views", &Handle::mse_views)
         .def("fwd", &Handle::fwd)
         .def("last_heap", &Handle::last_heap);
+    pybind11::class_<AdamWPlan>(m, "AdamWPlan")
+        .def(pybind11::init<int, uintptr_t, uintptr_t, uintptr_t, pybind11::list, pybind11::dict>())
+        .def("step", &AdamWPlan::step);
+    pybind11::class_<CacheHandle>(m, "CacheHandle")
+        .def(pybind11::init<uintptr_t, uintptr_t, uintptr_t, at::Tensor, at::Tensor, at::Tensor,
+                            at::Tensor, int64_t, int, std::vector<int32_t>, std::vector<int32_t>,
+                            int64_t>())
+        .def("append", &CacheHandle::append)
+        .def("window", &CacheHandle::window);
 }

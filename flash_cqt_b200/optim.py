@@ -12,6 +12,7 @@ holds a step advances them with every replay.
     opt.step()
 """
 import ctypes
+import sys
 
 import torch
 
@@ -40,6 +41,16 @@ def _same_order(a, b):
 
 def _reals(t):
     return t.numel() * (2 if t.is_complex() else 1)
+
+
+def _watched(opt):
+    """whether anyone listens to an optimizer's steps: hooks or a profiler"""
+    o = sys.modules[torch.optim.Optimizer.__module__]
+    return (getattr(torch.autograd.profiler, "_is_profiler_enabled", True)
+            or getattr(opt, "_optimizer_step_pre_hooks", True)
+            or getattr(opt, "_optimizer_step_post_hooks", True)
+            or getattr(o, "_global_optimizer_pre_hooks", True)
+            or getattr(o, "_global_optimizer_post_hooks", True))
 
 
 class AdamW(torch.optim.Optimizer):
@@ -93,7 +104,7 @@ class AdamW(torch.optim.Optimizer):
                                       state_bits=state_bits, master=master))
 
     def _reset(self):
-        self._dev = self._ws = self.grad_norm = None
+        self._dev = self._ws = self._plan = self.grad_norm = None
         self._retired = []
 
     def __getstate__(self):
@@ -104,6 +115,7 @@ class AdamW(torch.optim.Optimizer):
         self._reset()
         for g in self.param_groups:
             self._dev = g["params"][0].device if g["params"] else self._dev
+        self._total = sum(len(g["params"]) for g in self.param_groups)
 
     # ------------------------------------------------------------------ checks
     @staticmethod
@@ -152,20 +164,12 @@ class AdamW(torch.optim.Optimizer):
             if start < end:
                 raise ValueError("two parameters share memory, or one is given twice")
         super().add_param_group(group)
-        self._number()
+        self._total = sum(len(g["params"]) for g in self.param_groups)
 
     @staticmethod
     def _span(p):
         a = p.data_ptr()
         return [(a, a + p.numel() * p.element_size())] if p.numel() else []
-
-    def _number(self):
-        self._first = []
-        n = 0
-        for g in self.param_groups:
-            self._first.append(n)
-            n += len(g["params"])
-        self._total = n
 
     # ------------------------------------------------------------------- state
     def _new_state(self, p, g):
@@ -284,16 +288,51 @@ class AdamW(torch.optim.Optimizer):
                 self.grad_norm = torch.zeros((), dtype=torch.float32, device=self._dev)
         return self._ws
 
-    @torch.no_grad()
     def step(self, closure=None):
         """one step of every parameter that has a gradient; returns what
         ``closure`` (evaluated first, with gradients enabled) returns"""
+        if _watched(self):
+            return _hooked_step(self, closure)
+        return self._step(closure)
+
+    # the base class would wrap step() in its profiler label and hooks at every
+    # call (8 us); _watched() takes that way when there is one to serve
+    step.hooked = True
+
+    def _step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        if self._dev is None:
+            return loss
+        mod = _native.torch_ops()
+        if mod is None:
+            self._python_step()
+        elif self._plan is None or not self._plan_step():
+            # the first step, or states, parameters or groups were replaced
+            self._lists()
+            self._plan = mod.AdamWPlan(
+                self._dev.index, *[_native.fn_address(n) for n in (
+                    "cqt_grad_norm", "cqt_adamw_step", "cqt_last_error")],
+                self.param_groups, self.state)
+            if not self._plan_step():
+                raise RuntimeError("the optimizer's parameters changed during the step")
+        return loss
+
+    def _plan_step(self):
+        ws = self._workspace(self._total)
+        return self._plan.step(self.param_groups, self.state, self.max_norm, self.seed, ws,
+                               self.grad_norm)
+
+    @torch.no_grad()
+    def _lists(self):
+        """the tensors of every group that have gradients, as the library takes
+        them (states are made and checked), and the copies behind them"""
         lists, keep = [], []
-        for g, first in zip(self.param_groups, self._first):
+        first = 0
+        for g in self.param_groups:
+            self._check_options(g)
             todo = []
             for k, p in enumerate(g["params"]):
                 if p.grad is None or not p.numel():
@@ -309,12 +348,14 @@ class AdamW(torch.optim.Optimizer):
                     p.data_ptr(), grad.data_ptr(), at("master") if g["master"] else None,
                     at("exp_avg"), at("exp_avg_sq"), at("exp_avg_scale"), at("exp_avg_sq_scale"),
                     at("step"), _reals(p), _TYPES[p.dtype], first + k))
+            first += len(g["params"])
             lists.append((_native.CqtAdamwTensor * len(todo))(*todo))
-        if self._dev is None:
-            return loss
+        return lists, keep
+
+    def _python_step(self):
         with torch.cuda.device(self._dev):
+            lists, keep = self._lists()
             self._launch(lists)
-        return loss
 
     def _launch(self, lists):
         L, stream = _native.lib(), _raw_stream_of(self._dev.index)
@@ -335,3 +376,6 @@ class AdamW(torch.optim.Optimizer):
                 lr.data_ptr() if on_device else None, int(self.max_norm is not None), self.seed)
             _native._check(L.cqt_adamw_step(todo, len(todo), g["state_bits"], ctypes.byref(args),
                                             ws.data_ptr(), ws.numel(), stream), "cqt_adamw_step")
+
+
+_hooked_step = torch.optim.Optimizer.profile_hook_step(AdamW._step)

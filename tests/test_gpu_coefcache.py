@@ -99,6 +99,16 @@ def test_append_and_window(banks, bank, fmt):
         assert same(got, ring.window(6, end))
 
 
+def test_python_path(banks, monkeypatch):
+    """the calls through ctypes, as where the torch fast path is not built"""
+    from flash_cqt_b200 import _native
+    monkeypatch.setattr(_native, "_torchops", None)
+    monkeypatch.setattr(_native, "_torchops_tried", True)
+    test_append_and_window(banks, "short", "int8")
+    test_append_and_window(banks, "short", "e4m3")
+    test_views_and_orders(banks)
+
+
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 def test_special_values(banks, fmt):
     """not finite, tiny, huge, exact borders and ties"""

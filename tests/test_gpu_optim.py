@@ -430,6 +430,96 @@ def test_other_stream():
     assert torch.equal(p, q)
 
 
+@pytest.fixture
+def python_path(monkeypatch):
+    """the calls through ctypes, as where the torch fast path is not built"""
+    from flash_cqt_b200 import _native
+    monkeypatch.setattr(_native, "_torchops", None)
+    monkeypatch.setattr(_native, "_torchops_tried", True)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_python_path(bits, request):
+    def run():
+        ps = make([((300,), torch.float32), ((5, 77), torch.bfloat16), ((9,), torch.complex64)], seed=15)
+        opt = AdamW([dict(params=ps[:2], weight_decay=0.1), dict(params=ps[2:], lr=1e-3)], lr=1e-2,
+                    state_bits=bits, master=True, max_norm=0.5)
+        for _ in range(3):
+            opt.step()
+        return [p.detach() for p in ps] + [opt.grad_norm]
+    a = run()
+    request.getfixturevalue("python_path")
+    for x, y in zip(a, run()):
+        assert torch.equal(x, y)
+
+
+def test_replaced_state_is_seen():
+    """states, options and parameters that are exchanged between steps"""
+    def fresh():
+        p = make([((50,), torch.float32)], seed=16)[0]
+        return p, AdamW([p], lr=1e-2)
+    p, opt = fresh()
+    q, ref = fresh()
+    first = p.detach().clone()
+    opt.step()
+    for forget in (lambda: opt.state.clear(), lambda: opt.state.pop(p),
+                   lambda: opt.state.__setitem__(p, {})):
+        forget()
+        with torch.no_grad():
+            p.copy_(first)
+        opt.step()
+        assert int(opt.state[p]["step"]) == 1
+    opt.state[p]["exp_avg"] = torch.zeros_like(p)
+    opt.state[p]["exp_avg_sq"] = torch.zeros_like(p)
+    opt.state[p]["step"] = torch.zeros((), dtype=torch.int64, device=DEV)
+    with torch.no_grad():
+        p.copy_(first)
+    opt.step()
+    ref.step()
+    assert torch.equal(p, q)
+    p.data = torch.zeros(50, device=DEV)    # another storage of the same size
+    opt.step()
+    assert p.abs().max() > 0
+    opt.param_groups[0]["state_bits"] = 8   # does not fit the states
+    with pytest.raises(ValueError, match="exp_avg"):
+        opt.step()
+    opt.param_groups[0].update(state_bits=32, lr=-1.0)
+    with pytest.raises((ValueError, RuntimeError), match="lr"):
+        opt.step()
+
+
+def test_step_hooks_are_served():
+    p, calls = make([((5,), torch.float32)], seed=17)[0], []
+    opt = AdamW([p])
+    a = opt.register_step_pre_hook(lambda *_: calls.append("pre"))
+    opt.register_step_post_hook(lambda *_: calls.append("post"))
+    opt.step()
+    assert calls == ["pre", "post"] and int(opt.state[p]["step"]) == 1
+    a.remove()
+    opt.step()
+    assert calls == ["pre", "post", "post"] and int(opt.state[p]["step"]) == 2
+
+
+def test_deepcopy_and_save():
+    import io
+    p = make([((70,), torch.float32)], seed=18)[0]
+    opt = AdamW([p], lr=1e-2, max_norm=0.2, seed=3, state_bits=8)
+    opt.step()
+    f = io.BytesIO()   # (plain pickle cannot hold 8-bit tensors, torch.save can)
+    torch.save(opt, f)
+    f.seek(0)
+    for other in (copy.deepcopy(opt), torch.load(f, weights_only=False)):
+        q = other.param_groups[0]["params"][0]
+        if q.grad is None:
+            q.grad = p.grad.clone()
+        assert other.max_norm == 0.2 and other.seed == 3
+        other.step()
+        assert int(other.state[q]["step"]) == 2
+    q2 = q.detach().clone()
+    opt.step()
+    assert torch.equal(p, q2)
+
+
 def test_refusals():
     p = torch.zeros(8, device=DEV, requires_grad=True)
     with pytest.raises(ValueError, match="share memory"):
