@@ -78,7 +78,7 @@ class CoefCache:
         self.codes = z(*store, self.ncoef, 2).view(dt)
         self.scales = z(*store, self.ncoef // RUN).fill_(1).view(torch.float8_e8m0fnu)
         self.length = torch.zeros(self.lead, dtype=torch.int64, device=self.dev)
-        self._ws = z(256)
+        self._ws = z(max(4 * self.rows, 16))
         i32 = ctypes.c_int32 * len(self.gspec)
         self._bands, self._lens = i32(*[b for b, _ in self.gspec]), i32(*[M for _, M in self.gspec])
         self._desc = _native.CqtCache(

@@ -943,7 +943,7 @@ int cqt_sliced_adj_analysis(const cqt_tables* t, const float* gcoef, const cqt_s
 // CTA of each launch
 static size_t adamw_ws(int count) {
     const size_t launches = ((size_t)count + kOptTensors - 1) / kOptTensors;
-    return kWsHeader + launches * kOptCtas * sizeof(double);
+    return kWsHeader + launches * kNormCtas * sizeof(double);
 }
 
 size_t cqt_adamw_workspace_bytes(int count) { return count < 0 ? 0 : adamw_ws(count); }
@@ -1000,7 +1000,7 @@ static int take_tensors(const cqt_adamw_tensor* in, int count, int* at, OptTenso
         o.n = x.numel;
         o.chunk0 = 0;
         o.dtype = (short)x.dtype;
-        o.vec = (low & 15u) == 0 && codes;
+        o.vec = !codes || (low & 15u) ? 0 : ((low & 31u) ? 1 : 2);
         o.ordinal = x.ordinal;
     }
     return CQT_OK;
@@ -1083,7 +1083,7 @@ static int cache_args(const cqt_cache* c, const cqt_cache_part* parts, int slice
         return fail(CQT_ERR_ARG, "null or misaligned codes, scales or lengths");
     long long off = 0;
     gr->count = c->ngroups;
-    gr->wide = 1;
+    gr->wide = 2;
     for (int g = 0; g < kMaxGroups; ++g) {
         gr->data[g] = nullptr;
         gr->row[g] = gr->slice[g] = gr->band[g] = 0;
@@ -1106,7 +1106,9 @@ static int cache_args(const cqt_cache* c, const cqt_cache_part* parts, int slice
         if (c->rows > 0 && slices > 0 && (!p.data || (uintptr_t)p.data % 8))
             return fail(CQT_ERR_ARG, "null or misaligned coefficients");
         const long long strides = p.row_stride | p.slice_stride | p.band_stride;
-        if ((uintptr_t)p.data % 16 || (strides * item) % 16) gr->wide = 0;
+        const int align = (uintptr_t)p.data % 16 || (strides * item) % 16   ? 0
+                          : (uintptr_t)p.data % 32 || (strides * item) % 32 ? 1 : 2;
+        if (align < gr->wide) gr->wide = align;
     }
     if (!write && !gr->wide)
         return fail(CQT_ERR_ARG, "window outputs and their strides must be 16-byte aligned");
@@ -1118,8 +1120,7 @@ static int cache_args(const cqt_cache* c, const cqt_cache_part* parts, int slice
     st->capacity = c->capacity;
     st->ncoef = (int)off;
     st->int8 = c->format == CQT_CACHE_INT8;
-    // bounded before they are multiplied
-    if ((long long)slices * c->rows >= (1LL << 31) || cache_unit_count(*st, slices) >= (1LL << 31))
+    if ((long long)slices * c->rows >= (1LL << 31))
         return fail(CQT_ERR_ARG, "too many slices in one call");
     return CQT_OK;
 }

@@ -233,11 +233,27 @@ int band_twiddle_count();
 void band_twiddle_rows(float2* out, const float2* w2048);
 
 
+// 32 bytes in one access (sm_100): a warp whose lanes take 32 bytes each moves
+// whole sectors, where two 16-byte accesses would move every sector twice in
+// halves.  32-byte aligned addresses only.
+__device__ __forceinline__ void load_v8(const float* p, float (&x)[8]) {
+    asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]),
+                   "=f"(x[6]), "=f"(x[7])
+                 : "l"(p));
+}
+__device__ __forceinline__ void store_v8(float* p, const float (&x)[8]) {
+    asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(x[0]),
+                 "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
+                 : "memory");
+}
+
 // ---------------------------------------------------------------------------
 // AdamW over many tensors (optim.cu)
 constexpr int kOptBlock = 256;     // elements that share a scale (8-bit moments)
 constexpr int kOptTensors = 360;   // tensors in one launch (32 KB of kernel parameters)
-constexpr int kOptCtas = 148 * 4;  // CTAs of one launch at most
+constexpr int kOptCtas = 148 * 4;  // CTAs of one launch at most, of the step
+constexpr int kNormCtas = 148 * 7; // and of the norm
 enum OptType { kOptF32 = 0, kOptBf16 = 1, kOptF16 = 2 };
 
 struct OptTensor {
@@ -252,7 +268,7 @@ struct OptTensor {
     long long n;
     unsigned chunk0;       // first chunk of the tensor (filled in for the launch)
     short dtype;           // OptType
-    short vec;             // every array is aligned for 8 values at once
+    short vec;             // alignment of all arrays: 2 32 bytes, 1 16 bytes, 0 less
     int ordinal;           // the tensor's number in the rounding hash
 };
 
@@ -280,7 +296,7 @@ struct CacheStore {
     unsigned char* codes;      // [rows][capacity][ncoef][2]
     unsigned char* scales;     // [rows][capacity][ncoef / 16], exponent + 127
     long long* length;         // [rows] slices written so far
-    unsigned* ticket;          // zero between launches
+    unsigned* ticket;          // [rows], zero between launches
     int rows, capacity, ncoef;
     int int8;                  // 1: int8 codes, 0: e4m3
 };
@@ -294,11 +310,9 @@ struct CacheGroups {
     int off[kMaxGroups];       // heap offset of the group
     int shift[kMaxGroups];     // log2 of its block length
     int count;
-    int wide;                  // every quad is 16-byte aligned
+    int wide;                  // alignment of every run: 2 32 bytes, 1 16 bytes, 0 8 bytes
 };
 
-// units of work of a call (the caller keeps them below 2^31)
-long long cache_unit_count(const CacheStore& st, long long slices);
 cudaError_t launch_cache_append(const CacheStore& st, const CacheGroups& gr, int slices,
                                 const long long* counts, cudaStream_t s);
 cudaError_t launch_cache_window(const CacheStore& st, const CacheGroups& gr, int slices,

@@ -27,6 +27,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "internal.h"
 
@@ -56,10 +57,13 @@ __host__ __device__ __forceinline__ unsigned mix32(unsigned x) {
     return x ^ (x >> 16);
 }
 
-// ---- 8 consecutive values as 32-bit floats; `full`: all 8 are there and
-// aligned, else the first n of them one by one
-__device__ __forceinline__ void load8(const float* p, bool full, int n, float (&x)[8]) {
-    if (full) {
+// ---- 8 consecutive values as 32-bit floats.  `vec`: all 8 are there, at an
+// address that is a multiple of 32 (2) or 16 (1) bytes; else (0) the first n of
+// them one by one
+__device__ __forceinline__ void load8(const float* p, int vec, int n, float (&x)[8]) {
+    if (vec == 2) {
+        load_v8(p, x);
+    } else if (vec) {
         const float4 a = reinterpret_cast<const float4*>(p)[0];
         const float4 b = reinterpret_cast<const float4*>(p)[1];
         x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
@@ -69,8 +73,10 @@ __device__ __forceinline__ void load8(const float* p, bool full, int n, float (&
         for (int i = 0; i < 8; ++i) x[i] = i < n ? p[i] : 0.f;
     }
 }
-__device__ __forceinline__ void store8(float* p, bool full, int n, const float (&x)[8]) {
-    if (full) {
+__device__ __forceinline__ void store8(float* p, int vec, int n, const float (&x)[8]) {
+    if (vec == 2) {
+        store_v8(p, x);
+    } else if (vec) {
         reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
         reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
     } else {
@@ -81,63 +87,100 @@ __device__ __forceinline__ void store8(float* p, bool full, int n, const float (
 }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+// 16-bit parameters are rounded once, to nearest even, from the 32-bit result
 __device__ __forceinline__ void from_float(float x, __nv_bfloat16& y) { y = __float2bfloat16_rn(x); }
 __device__ __forceinline__ void from_float(float x, __half& y) { y = __float2half_rn(x); }
 template <class T>
-__device__ __forceinline__ void load8(const T* p, bool full, int n, float (&x)[8]) {
-    alignas(16) T h[8];
-    if (full) {
-        *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(p);
+__device__ __forceinline__ float2 pair_to_float(unsigned w) {
+    if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) {
+        return __half22float2(*reinterpret_cast<const __half2*>(&w));
+    } else {
+        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    }
+}
+template <class T>
+__device__ __forceinline__ unsigned pair_from_float(float a, float b) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const unsigned*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const unsigned*>(&h);
+    }
+}
+template <class T>
+__device__ __forceinline__ void load8(const T* p, int vec, int n, float (&x)[8]) {
+    if (vec) {
+        const uint4 w = *reinterpret_cast<const uint4*>(p);
+        const unsigned u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = to_float(h[i]);
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = pair_to_float<T>(u[i]);
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = i < n ? to_float(p[i]) : 0.f;
     }
 }
-// 16-bit parameters are rounded once, to nearest even, from the 32-bit result
 template <class T>
-__device__ __forceinline__ void store8(T* p, bool full, int n, const float (&x)[8]) {
-    alignas(16) T h[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) from_float(x[i], h[i]);
-    if (full) {
-        *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
+__device__ __forceinline__ void store8(T* p, int vec, int n, const float (&x)[8]) {
+    if (vec) {
+        *reinterpret_cast<uint4*>(p) =
+            make_uint4(pair_from_float<T>(x[0], x[1]), pair_from_float<T>(x[2], x[3]),
+                       pair_from_float<T>(x[4], x[5]), pair_from_float<T>(x[6], x[7]));
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (i < n) p[i] = h[i];
+            if (i < n) from_float(x[i], p[i]);
     }
 }
-__device__ __forceinline__ void load_codes(const uint8_t* p, bool full, int n, uint8_t (&c)[8]) {
-    if (full) {
-        *reinterpret_cast<uint2*>(c) = *reinterpret_cast<const uint2*>(p);
-    } else {
+// 8 codes, the first in the low byte of x
+__device__ __forceinline__ uint2 load_codes(const uint8_t* p, int vec, int n) {
+    if (vec) return *reinterpret_cast<const uint2*>(p);
+    uint2 c = make_uint2(0, 0);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) c[i] = i < n ? p[i] : 0;
-    }
+    for (int i = 0; i < 8; ++i)
+        if (i < n) (i < 4 ? c.x : c.y) |= (unsigned)p[i] << (8 * (i & 3));
+    return c;
 }
-__device__ __forceinline__ void store_codes(uint8_t* p, bool full, int n, const uint8_t (&c)[8]) {
-    if (full) {
-        *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(c);
+__device__ __forceinline__ void store_codes(uint8_t* p, int vec, int n, uint2 c) {
+    if (vec) {
+        *reinterpret_cast<uint2*>(p) = c;
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (i < n) p[i] = c[i];
+            if (i < n) p[i] = (uint8_t)((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
     }
 }
+__device__ __forceinline__ float sqrt_approx(float x) {
+    float y;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// the low bytes of 8 words
+__device__ __forceinline__ uint2 pack8(const unsigned (&c)[8]) {
+    return make_uint2(
+        __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410),
+        __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410));
+}
+// the values of 8 codes times s
 template <__nv_fp8_interpretation_t F>
-__device__ __forceinline__ void decode8(const uint8_t (&c)[8], uint8_t scale, float (&x)[8]) {
-    // 2^(scale - 127); a scale byte of 0 is the subnormal 2^-127
-    const float s = __uint_as_float(scale ? (unsigned)scale << 23 : 0x400000u);
+__device__ __forceinline__ void decode8(uint2 c, float s, float (&x)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        const __half2_raw h =
-            __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c[i] | c[i + 1] << 8), F);
+    for (int i = 0; i < 4; ++i) {
+        const unsigned w = i < 2 ? c.x : c.y;
+        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(
+            (__nv_fp8x2_storage_t)((i & 1) ? w >> 16 : w & 0xffffu), F);
         const float2 f = __half22float2(__half2(h));
-        x[i] = f.x * s;
-        x[i + 1] = f.y * s;
+        x[2 * i] = __fmul_rn(f.x, s);
+        x[2 * i + 1] = __fmul_rn(f.y, s);
     }
+}
+// 2^(byte - 127); a byte of 0 is the subnormal 2^-127
+__device__ __forceinline__ float scale_of(uint8_t byte) {
+    return __uint_as_float(byte ? (unsigned)byte << 23 : 0x400000u);
 }
 
 // what one step needs of one tensor's count: lr / (1 - b1^t), 1 / sqrt(1 -
@@ -146,40 +189,20 @@ struct StepScalars {
     float decay, rate, root, clip;
 };
 
-template <class T, int BITS>
-__device__ __forceinline__ void update8(const OptTensor& t, long long base, const OptArgs& a,
-                                        const StepScalars& s, unsigned key) {
-    const long long left = t.n - base;
-    const int n = left >= 8 ? 8 : (left > 0 ? (int)left : 0);
-    const bool full = n == 8 && t.vec;
-    float g[8], p[8], m[8], v[8];
-    load8(static_cast<const T*>(t.g) + base, full, n, g);
-    if (t.master) load8(t.master + base, full, n, p);
-    else load8(static_cast<const T*>(t.p) + base, full, n, p);
-    uint8_t mc[8], vc[8];
-    const long long block = base / kOptBlock;
-    if constexpr (BITS == 8) {
-        load_codes(static_cast<const uint8_t*>(t.m) + base, full, n, mc);
-        load_codes(static_cast<const uint8_t*>(t.v) + base, full, n, vc);
-        // a lane behind the tensor's end may be behind the scales' end too
-        decode8<__NV_E4M3>(mc, n > 0 ? t.ms[block] : 1, m);
-        decode8<__NV_E5M2>(vc, n > 0 ? t.vs[block] : 1, v);
-    } else {
-        load8(static_cast<const float*>(t.m) + base, full, n, m);
-        load8(static_cast<const float*>(t.v) + base, full, n, v);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float gi = __fmul_rn(g[i], s.clip);
-        m[i] = __fadd_rn(__fmul_rn(m[i], a.b1), __fmul_rn(gi, a.omb1));
-        v[i] = __fadd_rn(__fmul_rn(v[i], a.b2), __fmul_rn(__fmul_rn(gi, gi), a.omb2));
-        const float d = __fadd_rn(__fmul_rn(__fsqrt_rn(v[i]), s.root), a.eps);
-        p[i] = __fsub_rn(__fmul_rn(p[i], s.decay), __fmul_rn(__fdiv_rn(m[i], d), s.rate));
-    }
-    if (t.master) store8(t.master + base, full, n, p);
-    store8(static_cast<T*>(t.p) + base, full, n, p);
-    if constexpr (BITS == 8) {
-        unsigned mtop = 0, vtop = 0;
+// New 8-bit moments of one lane's 8 elements, the first n of them real.  The
+// scales follow from the largest values of the warp's 256.
+//
+// RARE: some moment of the block is not finite, or a scale is the largest
+// there is.  Values that are not finite then do not count for the scale and
+// get the formats' own codes; and a value next to 2^128 does not round up to
+// it (code 119 is 240 in e4m3 and 1.75 * 2^14 in e5m2).
+template <bool RARE>
+__device__ __forceinline__ void encode_moments(const float (&m)[8], const float (&v)[8], int n,
+                                               unsigned mtop, unsigned vtop, unsigned index,
+                                               unsigned key, uint2& mc, uint2& vc, int& mk,
+                                               int& vk) {
+    if constexpr (RARE) {
+        mtop = vtop = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const unsigned mb = __float_as_uint(m[i]) & 0x7fffffffu;
@@ -189,28 +212,97 @@ __device__ __forceinline__ void update8(const OptTensor& t, long long base, cons
         }
         mtop = __reduce_max_sync(0xffffffffu, mtop);
         vtop = __reduce_max_sync(0xffffffffu, vtop);
-        // 448 = 1.75 * 2^8 and 57344 = 1.75 * 2^15: the exponent of the
-        // largest value, one more where its fraction is above 1.75
-        const int mk = max(1, (int)((mtop + 0x1fffffu) >> 23) - 8);
-        const int vk = max(1, (int)((vtop + 0x1fffffu) >> 23) - 15);
-        // at the largest scales a value next to 2^128 must not round up to it:
-        // code 119 is 240 in e4m3 and 1.75 * 2^14 in e5m2
-        const int mmost = mk == 247 ? 119 : 126, vmost = vk == 240 ? 119 : 123;
-        const float mi = __uint_as_float((unsigned)(254 - mk) << 23);
-        const float vi = __uint_as_float((unsigned)(254 - vk) << 23);
+    }
+    // 448 = 1.75 * 2^8 and 57344 = 1.75 * 2^15: the exponent of the largest
+    // value, one more where its fraction is above 1.75
+    mk = max(1, (int)((mtop + 0x1fffffu) >> 23) - 8);
+    vk = max(1, (int)((vtop + 0x1fffffu) >> 23) - 15);
+    const float mi = __uint_as_float((unsigned)(254 - mk) << 23);
+    const float vi = __uint_as_float((unsigned)(254 - vk) << 23);
+    unsigned a[8], b[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        // the noise goes in below the last bit that is kept; the exponent's
+        // bias changes with the same addition
+        const unsigned h = mix32((index + i) ^ key);
+        const unsigned mb = __float_as_uint(__fmul_rn(m[i], mi));
+        const unsigned vb = __float_as_uint(__fmul_rn(v[i], vi));
+        int c = (int)((mb & 0x7fffffffu) + ((h << 4) & 0xffff0u) + (8u - (120u << 23))) >> 20;
+        int d = (int)(vb + ((h >> 11) & 0x1fffe0u) + (16u - (112u << 23))) >> 21;
+        d = max(d, 4);
+        if constexpr (RARE) {
+            c = min(c, mk == 247 ? 119 : 126);
+            d = min(d, vk == 240 ? 119 : 123);
+        }
+        a[i] = (unsigned)(c < 8 ? 0 : c) | ((mb >> 24) & 0x80u);
+        b[i] = v[i] > 0.f ? (unsigned)d : 0u;
+        if constexpr (RARE) {
+            const unsigned vr = __float_as_uint(v[i]) & 0x7fffffffu;
+            if ((__float_as_uint(m[i]) & 0x7fffffffu) >= 0x7f800000u) a[i] = 0x7fu;
+            if (vr >= 0x7f800000u) b[i] = vr == 0x7f800000u ? 0x7cu : 0x7fu;
+        }
+    }
+    mc = pack8(a);
+    vc = pack8(b);
+}
+
+template <class T, int BITS>
+__device__ __forceinline__ void update8(const OptTensor& t, long long base, const OptArgs& a,
+                                        const StepScalars& s, unsigned key) {
+    const long long left = t.n - base;
+    const int n = left >= 8 ? 8 : (left > 0 ? (int)left : 0);
+    const int full = n == 8 ? t.vec : 0;
+    float g[8], p[8], m[8], v[8];
+    load8(static_cast<const T*>(t.g) + base, full, n, g);
+    if (t.master) load8(t.master + base, full, n, p);
+    else load8(static_cast<const T*>(t.p) + base, full, n, p);
+    const long long block = base / kOptBlock;
+    if constexpr (BITS == 8) {
+        const uint2 mc = load_codes(static_cast<const uint8_t*>(t.m) + base, full, n);
+        const uint2 vc = load_codes(static_cast<const uint8_t*>(t.v) + base, full, n);
+        // a lane behind the tensor's end may be behind the scales' end too.
+        // The scales are powers of two: b (code s) = code (b s)
+        const float ms = scale_of(n > 0 ? t.ms[block] : 1), vs = scale_of(n > 0 ? t.vs[block] : 1);
+        decode8<__NV_E4M3>(mc, __fmul_rn(ms, a.b1), m);
+        decode8<__NV_E5M2>(vc, __fmul_rn(vs, a.b2), v);
+    } else {
+        load8(static_cast<const float*>(t.m) + base, full, n, m);
+        load8(static_cast<const float*>(t.v) + base, full, n, v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const unsigned h = mix32((unsigned)(base + i) ^ key);
-            const unsigned mb = __float_as_uint(__fmul_rn(m[i], mi));
-            int c = (int)(((mb & 0x7fffffffu) + ((h & 0xffffu) << 4) + 8u) >> 20) - (120 << 3);
-            c = (c < 8 ? 0 : min(c, mmost)) | (int)((mb >> 24) & 0x80u);
-            mc[i] = (__float_as_uint(m[i]) & 0x7fffffffu) < 0x7f800000u ? (uint8_t)c : 0x7f;
-            const unsigned vb = __float_as_uint(__fmul_rn(v[i], vi));
-            c = (int)((vb + ((h >> 16) << 5) + 16u) >> 21) - (112 << 2);
-            c = v[i] > 0.f ? min(max(c, 4), vmost) : 0;
-            const unsigned vr = __float_as_uint(v[i]) & 0x7fffffffu;
-            vc[i] = vr < 0x7f800000u ? (uint8_t)c : (vr == 0x7f800000u ? 0x7c : 0x7f);
+            m[i] = __fmul_rn(m[i], a.b1);
+            v[i] = __fmul_rn(v[i], a.b2);
         }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float gi = __fmul_rn(g[i], s.clip);
+        m[i] = __fadd_rn(m[i], __fmul_rn(gi, a.omb1));
+        v[i] = __fadd_rn(v[i], __fmul_rn(__fmul_rn(gi, gi), a.omb2));
+        // root and quotient to 2^-22: their last bits are far below the
+        // update's own, and correctly rounded ones take half of the instructions
+        const float d = __fadd_rn(__fmul_rn(sqrt_approx(v[i]), s.root), a.eps);
+        p[i] = __fsub_rn(__fmul_rn(p[i], s.decay), __fmul_rn(__fdividef(m[i], d), s.rate));
+    }
+    if (t.master) store8(t.master + base, full, n, p);
+    store8(static_cast<T*>(t.p) + base, full, n, p);
+    if constexpr (BITS == 8) {
+        // elements behind the end are zeros: they change no maximum
+        unsigned mtop = 0, vtop = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            mtop = max(mtop, __float_as_uint(m[i]) & 0x7fffffffu);
+            vtop = max(vtop, __float_as_uint(v[i]) & 0x7fffffffu);
+        }
+        mtop = __reduce_max_sync(0xffffffffu, mtop);
+        vtop = __reduce_max_sync(0xffffffffu, vtop);
+        uint2 mc, vc;
+        int mk, vk;
+        // above 1.75 * 2^127 the scales are the largest (or there is none)
+        if (max(mtop, vtop) > 0x7f600000u)
+            encode_moments<true>(m, v, n, mtop, vtop, (unsigned)base, key, mc, vc, mk, vk);
+        else
+            encode_moments<false>(m, v, n, mtop, vtop, (unsigned)base, key, mc, vc, mk, vk);
         store_codes(static_cast<uint8_t*>(t.m) + base, full, n, mc);
         store_codes(static_cast<uint8_t*>(t.v) + base, full, n, vc);
         if ((threadIdx.x & 31) == 0 && n > 0) {
@@ -235,35 +327,54 @@ __device__ __forceinline__ int find_tensor(const OptTable<N>& tab, unsigned c) {
     return lo;
 }
 
+struct ChunkPlan {
+    int tensor;
+    float rate, root;
+    unsigned key;
+};
+
 template <int N, int BITS>
 __global__ void __launch_bounds__(kThreads)
 adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ OptArgs a) {
-    StepScalars s{};
-    unsigned key = 0;
-    int cur = -1;
+    __shared__ ChunkPlan plan[kThreads];
     const double lr = a.lr_dev ? (double)*a.lr_dev : a.lr;
+    StepScalars s{};
     s.decay = (float)(1.0 - lr * a.wd);
     s.clip = 1.f;
     if (a.norm) {
         const double c = a.max_norm / (*a.norm + 1e-6);
         s.clip = c > 1.0 ? 1.f : (float)c;   // NaN stays NaN
     }
-    for (unsigned c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
-        const int i = find_tensor(tab, c);
-        const OptTensor& t = tab.t[i];
-        const long long base = (long long)(c - t.chunk0) * kChunk + threadIdx.x * kLane;
-        if (i != cur) {
-            cur = i;
-            const double step = (double)(*t.step + 1);
-            s.rate = (float)(lr / (1.0 - exp2(step * a.lb1)));
-            s.root = (float)(1.0 / sqrt(1.0 - exp2(step * a.lb2)));
+    // the CTA's chunks are one grid apart (neighbouring CTAs share DRAM pages).
+    // What each of them needs of its tensor -- which one it is, powers of the
+    // betas in 64 bits -- is worked out by one thread a chunk, a CTA's width of
+    // chunks at a time
+    for (unsigned c0 = blockIdx.x; c0 < tab.chunks; c0 += kThreads * gridDim.x) {
+        __syncthreads();
+        const unsigned long long mine = c0 + (unsigned long long)threadIdx.x * gridDim.x;
+        if (mine < tab.chunks) {
+            ChunkPlan q;
+            q.tensor = find_tensor(tab, (unsigned)mine);
+            const OptTensor& t = tab.t[q.tensor];
+            const long long step = *t.step + 1;
+            q.rate = (float)(lr / (1.0 - exp2((double)step * a.lb1)));
+            q.root = (float)(1.0 / sqrt(1.0 - exp2((double)step * a.lb2)));
+            q.key = BITS == 8 ? mix32(mix32(a.seed_key + (unsigned)step) + (unsigned)t.ordinal) : 0;
+            plan[threadIdx.x] = q;
         }
-        if constexpr (BITS == 8)
-            key = mix32(mix32(mix32(a.seed_key + (unsigned)(*t.step + 1)) + (unsigned)t.ordinal) +
-                        (unsigned)(base >> 32));
-        if (t.dtype == kOptF32) update8<float, BITS>(t, base, a, s, key);
-        else if (t.dtype == kOptBf16) update8<__nv_bfloat16, BITS>(t, base, a, s, key);
-        else update8<__half, BITS>(t, base, a, s, key);
+        __syncthreads();
+        unsigned c = c0;
+        for (int k = 0; k < kThreads && c < tab.chunks; ++k, c += gridDim.x) {
+            const ChunkPlan q = plan[k];
+            const OptTensor& t = tab.t[q.tensor];
+            const long long base = (long long)(c - t.chunk0) * kChunk + threadIdx.x * kLane;
+            s.rate = q.rate;
+            s.root = q.root;
+            const unsigned key = BITS == 8 ? mix32(q.key + (unsigned)(base >> 32)) : 0;
+            if (t.dtype == kOptF32) update8<float, BITS>(t, base, a, s, key);
+            else if (t.dtype == kOptBf16) update8<__nv_bfloat16, BITS>(t, base, a, s, key);
+            else update8<__half, BITS>(t, base, a, s, key);
+        }
     }
     // every CTA has read the counts it needs: the last one to come here
     // advances them
@@ -279,15 +390,14 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
 // ---- sqrt(sum of squares over all gradients), summed in 64 bits in a fixed
 // order: threads, warps, CTAs, launches
 template <class T>
-__device__ __forceinline__ double squares8(const void* p, long long base, long long size, bool vec) {
+__device__ __forceinline__ void squares8(const T* p, long long base, long long size, int vec,
+                                         double (&sum)[4]) {
     const long long left = size - base;
     const int n = left >= 8 ? 8 : (left > 0 ? (int)left : 0);
     float x[8];
-    load8(static_cast<const T*>(p) + base, n == 8 && vec, n, x);
-    double sum = 0;
+    load8(p + base, n == 8 ? vec : 0, n, x);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum = fma((double)x[i], (double)x[i], sum);
-    return sum;
+    for (int i = 0; i < 8; ++i) sum[i & 3] = fma((double)x[i], (double)x[i], sum[i & 3]);
 }
 
 __device__ __forceinline__ double cta_sum(double x) {
@@ -306,14 +416,25 @@ template <int N>
 __global__ void __launch_bounds__(kThreads)
 norm_kernel(const __grid_constant__ OptTable<N> tab, double* partial, int first, int last,
             unsigned* ticket, double* norm, float* norm32) {
-    double sum = 0;
-    for (unsigned c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
-        const OptTensor& t = tab.t[find_tensor(tab, c)];
-        const long long base = (long long)(c - t.chunk0) * kChunk + threadIdx.x * kLane;
-        if (t.dtype == kOptF32) sum += squares8<float>(t.g, base, t.n, t.vec);
-        else if (t.dtype == kOptBf16) sum += squares8<__nv_bfloat16>(t.g, base, t.n, t.vec);
-        else sum += squares8<__half>(t.g, base, t.n, t.vec);
+    __shared__ int tensor[kThreads];   // of the CTA's next chunks, as above
+    double part[4] = {0, 0, 0, 0};
+    for (unsigned c0 = blockIdx.x; c0 < tab.chunks; c0 += kThreads * gridDim.x) {
+        __syncthreads();
+        const unsigned long long mine = c0 + (unsigned long long)threadIdx.x * gridDim.x;
+        if (mine < tab.chunks) tensor[threadIdx.x] = find_tensor(tab, (unsigned)mine);
+        __syncthreads();
+        unsigned c = c0;
+#pragma unroll 2
+        for (int k = 0; k < kThreads && c < tab.chunks; ++k, c += gridDim.x) {
+            const OptTensor& t = tab.t[tensor[k]];
+            const long long base = (long long)(c - t.chunk0) * kChunk + threadIdx.x * kLane;
+            if (t.dtype == kOptF32) squares8(static_cast<const float*>(t.g), base, t.n, t.vec, part);
+            else if (t.dtype == kOptBf16)
+                squares8(static_cast<const __nv_bfloat16*>(t.g), base, t.n, t.vec, part);
+            else squares8(static_cast<const __half*>(t.g), base, t.n, t.vec, part);
+        }
     }
+    double sum = (part[0] + part[1]) + (part[2] + part[3]);
     sum = cta_sum(sum);
     __shared__ unsigned order;
     if (threadIdx.x == 0) {
@@ -336,9 +457,8 @@ norm_kernel(const __grid_constant__ OptTable<N> tab, double* partial, int first,
     }
 }
 
-// CTAs of one launch: all chunks at once up to four CTAs an SM, then a loop
-unsigned opt_grid(unsigned chunks) {
-    const unsigned most = kOptCtas;
+// CTAs of one launch: all chunks at once up to what the SMs hold, then a loop
+unsigned opt_grid(unsigned chunks, unsigned most) {
     return chunks < 1 ? 1 : (chunks < most ? chunks : most);
 }
 
@@ -358,7 +478,7 @@ template <int N>
 cudaError_t adamw_part(const OptTensor* t, int count, int bits, const OptArgs& a, cudaStream_t s) {
     OptTable<N> tab;
     fill(&tab, t, count);
-    const unsigned grid = opt_grid(tab.chunks);
+    const unsigned grid = opt_grid(tab.chunks, kOptCtas);
     if (bits == 8) adamw_kernel<N, 8><<<grid, kThreads, 0, s>>>(tab, a);
     else adamw_kernel<N, 32><<<grid, kThreads, 0, s>>>(tab, a);
     return cudaGetLastError();
@@ -369,7 +489,7 @@ cudaError_t norm_part(const OptTensor* t, int count, double* partial, int* first
                       unsigned* ticket, double* norm, float* norm32, cudaStream_t s) {
     OptTable<N> tab;
     fill(&tab, t, count);
-    const unsigned grid = opt_grid(tab.chunks);
+    const unsigned grid = opt_grid(tab.chunks, kNormCtas);
     norm_kernel<N><<<grid, kThreads, 0, s>>>(tab, partial, *first, last ? 1 : 0, ticket, norm,
                                              norm32);
     *first += (int)grid;

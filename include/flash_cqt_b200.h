@@ -374,7 +374,7 @@ typedef struct cqt_cache {
     void* codes;                /* [rows][capacity][ncoef][2], 16-byte aligned */
     uint8_t* scales;            /* [rows][capacity][ncoef / 16] */
     int64_t* length;            /* device [rows]: slices written so far */
-    void* workspace;            /* 256 bytes, zeroed once */
+    void* workspace;            /* 4 bytes a row, 16-byte aligned, zeroed once */
     int32_t rows, capacity;
     int32_t format;             /* CQT_CACHE_INT8 or CQT_CACHE_E4M3 */
     int32_t ngroups;            /* <= 16 */
