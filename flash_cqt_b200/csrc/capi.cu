@@ -958,9 +958,11 @@ static int check_adamw_ws(int count, void* ws, size_t bytes) {
 
 static bool opt_type(int32_t d) { return d == CQT_F32 || d == CQT_BF16 || d == CQT_F16; }
 
-// the next tensors of the list that hold elements, at most kOptTensors of them
+// the next tensors of the list that hold elements, at most kOptTensors of them;
+// kind: only those of one type, with a master copy or without (-1: all of them)
+static int opt_kind(const cqt_adamw_tensor& x) { return 2 * x.dtype + (x.master ? 1 : 0); }
 static int take_tensors(const cqt_adamw_tensor* in, int count, int* at, OptTensor* out, int* n,
-                        bool grads_only, int bits) {
+                        bool grads_only, int bits, int kind) {
     static_assert(kOptF32 == CQT_F32 && kOptBf16 == CQT_BF16 && kOptF16 == CQT_F16, "types");
     long long chunks = 0;
     *n = 0;
@@ -968,7 +970,7 @@ static int take_tensors(const cqt_adamw_tensor* in, int count, int* at, OptTenso
         const cqt_adamw_tensor& x = in[*at];
         if (x.numel < 0 || !opt_type(x.dtype))
             return fail(CQT_ERR_ARG, "bad tensor (numel >= 0, a known dtype)");
-        if (x.numel == 0) continue;
+        if (x.numel == 0 || (kind >= 0 && opt_kind(x) != kind)) continue;
         const uintptr_t item = x.dtype == CQT_F32 ? 4 : 2;
         if (!x.grad || (uintptr_t)x.grad % item)
             return fail(CQT_ERR_ARG, "null or misaligned gradient");
@@ -1016,7 +1018,7 @@ int cqt_grad_norm(const cqt_adamw_tensor* tensors, int count, float* norm, void*
     OptTensor part[kOptTensors];
     int at = 0, n = 0, first = 0;
     do {   // a list without elements has the norm 0: one launch in any case
-        if (int rc = take_tensors(tensors, count, &at, part, &n, true, 32)) return rc;
+        if (int rc = take_tensors(tensors, count, &at, part, &n, true, 32, -1)) return rc;
         bool last = true;
         for (int i = at; i < count; ++i) last = last && tensors[i].numel == 0;
         const cudaError_t e = launch_grad_norm(
@@ -1056,12 +1058,22 @@ int cqt_adamw_step(const cqt_adamw_tensor* tensors, int count, int state_bits,
     o.eps = (float)a->eps;
     o.seed_key = a->seed;
     OptTensor part[kOptTensors];
-    for (int at = 0, n = 0; at < count;) {
-        if (int rc = take_tensors(tensors, count, &at, part, &n, false, state_bits)) return rc;
-        if (n == 0) break;
-        const cudaError_t e =
-            launch_adamw(part, n, state_bits, o, static_cast<cudaStream_t>(stream));
-        if (e != cudaSuccess) return cuda_fail(e, "adamw launch");
+    unsigned kinds = 0;   // of the tensors that hold elements
+    for (int at = 0, n = 0; at < count;) {   // all are checked before the first is changed
+        if (int rc = take_tensors(tensors, count, &at, part, &n, false, state_bits, -1)) return rc;
+    }
+    for (int i = 0; i < count; ++i)
+        if (tensors[i].numel) kinds |= 1u << opt_kind(tensors[i]);
+    for (int kind = 0; kind < 6; ++kind) {
+        if (!(kinds >> kind & 1)) continue;
+        for (int at = 0, n = 0; at < count;) {
+            if (int rc = take_tensors(tensors, count, &at, part, &n, false, state_bits, kind))
+                return rc;
+            if (n == 0) break;
+            const cudaError_t e =
+                launch_adamw(part, n, state_bits, o, static_cast<cudaStream_t>(stream));
+            if (e != cudaSuccess) return cuda_fail(e, "adamw launch");
+        }
     }
     return CQT_OK;
 }

@@ -252,8 +252,7 @@ __device__ __forceinline__ void store_v8(float* p, const float (&x)[8]) {
 // AdamW over many tensors (optim.cu)
 constexpr int kOptBlock = 256;     // elements that share a scale (8-bit moments)
 constexpr int kOptTensors = 360;   // tensors in one launch (32 KB of kernel parameters)
-constexpr int kOptCtas = 148 * 4;  // CTAs of one launch at most, of the step
-constexpr int kNormCtas = 148 * 7; // and of the norm
+constexpr int kNormCtas = 148 * 7; // CTAs of one launch of the norm at most
 enum OptType { kOptF32 = 0, kOptBf16 = 1, kOptF16 = 2 };
 
 struct OptTensor {
@@ -282,7 +281,8 @@ struct OptArgs {
     unsigned seed_key;
 };
 
-// one launch over at most kOptTensors tensors
+// one launch over 1 to kOptTensors tensors of one type, all with a master copy
+// or none
 cudaError_t launch_adamw(const OptTensor* t, int count, int bits, OptArgs a, cudaStream_t s);
 // one launch of norm = sqrt(sum of the squares of all gradients): the sums of
 // its CTAs go to partial[*first ...], and the last launch adds them all up

@@ -49,28 +49,60 @@ struct OptTable {
 
 // shifts and odd multipliers (the fractional bits of the square roots of 2
 // and 3); every bit of the input reaches every bit of the output
-__host__ __device__ __forceinline__ unsigned mix32(unsigned x) {
-    x ^= x >> 16;
+__host__ __device__ __forceinline__ unsigned mix_first(unsigned x) { return x ^ (x >> 16); }
+__host__ __device__ __forceinline__ unsigned mix_middle(unsigned x) {
     x *= 0x6A09E667u;
     x ^= x >> 15;
-    x *= 0xBB67AE85u;
+    return x * 0xBB67AE85u;
+}
+__host__ __device__ __forceinline__ unsigned mix32(unsigned x) {
+    x = mix_middle(mix_first(x));
     return x ^ (x >> 16);
 }
 
-// ---- 8 consecutive values as 32-bit floats.  `vec`: all 8 are there, at an
-// address that is a multiple of 32 (2) or 16 (1) bytes; else (0) the first n of
-// them one by one
-__device__ __forceinline__ void load8(const float* p, int vec, int n, float (&x)[8]) {
+// the larger of two, NaN if either is
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
+// ---- 8 consecutive values.  `vec`: all 8 are there, at an address that is a
+// multiple of 32 (2) or 16 (1) bytes; else (0) the first n of them one by one,
+// zeros behind.  They stay as loaded (Raw8) until they are needed: a load waits
+// for nothing.
+template <class T>
+struct Raw8 {
+    uint4 w;
+};
+template <>
+struct Raw8<float> {
+    float f[8];
+};
+__device__ __forceinline__ void load8(const float* p, int vec, int n, Raw8<float>& x) {
     if (vec == 2) {
-        load_v8(p, x);
+        load_v8(p, x.f);
     } else if (vec) {
         const float4 a = reinterpret_cast<const float4*>(p)[0];
         const float4 b = reinterpret_cast<const float4*>(p)[1];
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+        x.f[0] = a.x; x.f[1] = a.y; x.f[2] = a.z; x.f[3] = a.w;
+        x.f[4] = b.x; x.f[5] = b.y; x.f[6] = b.z; x.f[7] = b.w;
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = i < n ? p[i] : 0.f;
+        for (int i = 0; i < 8; ++i) x.f[i] = i < n ? p[i] : 0.f;
+    }
+}
+template <class T>
+__device__ __forceinline__ void load8(const T* p, int vec, int n, Raw8<T>& x) {
+    if (vec) {
+        x.w = *reinterpret_cast<const uint4*>(p);
+    } else {
+        const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+        unsigned w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) w[i / 2] |= (unsigned)h[i] << (16 * (i & 1));
+        x.w = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 __device__ __forceinline__ void store8(float* p, int vec, int n, const float (&x)[8]) {
@@ -85,14 +117,12 @@ __device__ __forceinline__ void store8(float* p, int vec, int n, const float (&x
             if (i < n) p[i] = x[i];
     }
 }
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 // 16-bit parameters are rounded once, to nearest even, from the 32-bit result
 __device__ __forceinline__ void from_float(float x, __nv_bfloat16& y) { y = __float2bfloat16_rn(x); }
 __device__ __forceinline__ void from_float(float x, __half& y) { y = __float2half_rn(x); }
 template <class T>
 __device__ __forceinline__ float2 pair_to_float(unsigned w) {
-    if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) {
+    if constexpr (std::is_same<T, __half>::value) {
         return __half22float2(*reinterpret_cast<const __half2*>(&w));
     } else {
         return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
@@ -108,20 +138,18 @@ __device__ __forceinline__ unsigned pair_from_float(float a, float b) {
         return *reinterpret_cast<const unsigned*>(&h);
     }
 }
+__device__ __forceinline__ void unpack(const Raw8<float>& r, float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = r.f[i];
+}
 template <class T>
-__device__ __forceinline__ void load8(const T* p, int vec, int n, float (&x)[8]) {
-    if (vec) {
-        const uint4 w = *reinterpret_cast<const uint4*>(p);
-        const unsigned u[4] = {w.x, w.y, w.z, w.w};
+__device__ __forceinline__ void unpack(const Raw8<T>& r, float (&x)[8]) {
+    const unsigned u[4] = {r.w.x, r.w.y, r.w.z, r.w.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = pair_to_float<T>(u[i]);
-            x[2 * i] = f.x;
-            x[2 * i + 1] = f.y;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = i < n ? to_float(p[i]) : 0.f;
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = pair_to_float<T>(u[i]);
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
     }
 }
 template <class T>
@@ -154,16 +182,29 @@ __device__ __forceinline__ void store_codes(uint8_t* p, int vec, int n, uint2 c)
             if (i < n) p[i] = (uint8_t)((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
     }
 }
-__device__ __forceinline__ float sqrt_approx(float x) {
+// sqrt(max(x, 2^-126)) and a / b to 2^-22
+__device__ __forceinline__ float root_of(float x) {
     float y;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(max_nan(x, 0x1p-126f)));
     return y;
 }
-// the low bytes of 8 words
-__device__ __forceinline__ uint2 pack8(const unsigned (&c)[8]) {
-    return make_uint2(
-        __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410),
-        __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410));
+__device__ __forceinline__ float quotient(float a, float b) {
+    float y;
+    asm("div.approx.ftz.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+// 8 values to codes, the first in the low byte
+template <__nv_fp8_interpretation_t F>
+__device__ __forceinline__ uint2 to_fp8(const float (&x)[8]) {
+    unsigned w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        w[i] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * i], x[2 * i + 1]), __NV_SATFINITE, F);
+    return make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+}
+__device__ __forceinline__ void put_byte(uint2& c, int i, unsigned byte) {
+    unsigned& w = i < 4 ? c.x : c.y;
+    w = (w & ~(0xffu << (8 * (i & 3)))) | byte << (8 * (i & 3));
 }
 // the values of 8 codes times s
 template <__nv_fp8_interpretation_t F>
@@ -189,13 +230,17 @@ struct StepScalars {
     float decay, rate, root, clip;
 };
 
-// New 8-bit moments of one lane's 8 elements, the first n of them real.  The
-// scales follow from the largest values of the warp's 256.
+// New 8-bit moments of one lane's 8 elements, the first n of them real, from
+// the largest magnitudes of the warp's 256 (NaN where one of them is).
+//
+// A value over its scale gets its noise added below the last bit that is kept,
+// as integers, and the bits below that cut off: the conversion to 8 bits then
+// rounds nothing.
 //
 // RARE: some moment of the block is not finite, or a scale is the largest
 // there is.  Values that are not finite then do not count for the scale and
 // get the formats' own codes; and a value next to 2^128 does not round up to
-// it (code 119 is 240 in e4m3 and 1.75 * 2^14 in e5m2).
+// it (it stays at 240 in e4m3 and at 1.75 * 2^14 in e5m2).
 template <bool RARE>
 __device__ __forceinline__ void encode_moments(const float (&m)[8], const float (&v)[8], int n,
                                                unsigned mtop, unsigned vtop, unsigned index,
@@ -219,55 +264,90 @@ __device__ __forceinline__ void encode_moments(const float (&m)[8], const float 
     vk = max(1, (int)((vtop + 0x1fffffu) >> 23) - 15);
     const float mi = __uint_as_float((unsigned)(254 - mk) << 23);
     const float vi = __uint_as_float((unsigned)(254 - vk) << 23);
-    unsigned a[8], b[8];
+    // mix32 of (index + i) ^ key for i < 8, index a multiple of 8: its first
+    // step is the same for all of them
+    const unsigned first = mix_first(index ^ key);
+    float a[8], b[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        // the noise goes in below the last bit that is kept; the exponent's
-        // bias changes with the same addition
-        const unsigned h = mix32((index + i) ^ key);
-        const unsigned mb = __float_as_uint(__fmul_rn(m[i], mi));
-        const unsigned vb = __float_as_uint(__fmul_rn(v[i], vi));
-        int c = (int)((mb & 0x7fffffffu) + ((h << 4) & 0xffff0u) + (8u - (120u << 23))) >> 20;
-        int d = (int)(vb + ((h >> 11) & 0x1fffe0u) + (16u - (112u << 23))) >> 21;
-        d = max(d, 4);
+        const unsigned h = mix_middle(first ^ i);
+        // the low and the high half of mix32's result (its last step folds the
+        // high half into the low one)
+        const unsigned hm = ((h << 4) ^ (h >> 12)) & 0xffff0u, hv = (h >> 11) & 0x1fffe0u;
+        const unsigned mb = __float_as_uint(__fmul_rn(m[i], mi)) + hm + 8u;
+        const unsigned vb = __float_as_uint(__fmul_rn(v[i], vi)) + hv + 16u;
+        a[i] = __uint_as_float(mb & 0xfff00000u);
+        b[i] = __uint_as_float(vb & 0xffe00000u);
         if constexpr (RARE) {
-            c = min(c, mk == 247 ? 119 : 126);
-            d = min(d, vk == 240 ? 119 : 123);
+            const float mmost = mk == 247 ? 240.f : 448.f, vmost = vk == 240 ? 28672.f : 57344.f;
+            a[i] = fminf(fmaxf(a[i], -mmost), mmost);
+            b[i] = fminf(b[i], vmost);
         }
-        a[i] = (unsigned)(c < 8 ? 0 : c) | ((mb >> 24) & 0x80u);
-        b[i] = v[i] > 0.f ? (unsigned)d : 0u;
-        if constexpr (RARE) {
+        // below the smallest normal value: 0 for m, that value for v
+        if (!(fabsf(a[i]) >= 0x1p-6f)) a[i] = 0.f;
+        b[i] = v[i] > 0.f ? fmaxf(b[i], 0x1p-14f) : 0.f;
+    }
+    mc = to_fp8<__NV_E4M3>(a);
+    vc = to_fp8<__NV_E5M2>(b);
+    if constexpr (RARE) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
             const unsigned vr = __float_as_uint(v[i]) & 0x7fffffffu;
-            if ((__float_as_uint(m[i]) & 0x7fffffffu) >= 0x7f800000u) a[i] = 0x7fu;
-            if (vr >= 0x7f800000u) b[i] = vr == 0x7f800000u ? 0x7cu : 0x7fu;
+            if ((__float_as_uint(m[i]) & 0x7fffffffu) >= 0x7f800000u) put_byte(mc, i, 0x7fu);
+            if (vr >= 0x7f800000u) put_byte(vc, i, vr == 0x7f800000u ? 0x7cu : 0x7fu);
         }
     }
-    mc = pack8(a);
-    vc = pack8(b);
 }
 
-template <class T, int BITS>
-__device__ __forceinline__ void update8(const OptTensor& t, long long base, const OptArgs& a,
-                                        const StepScalars& s, unsigned key) {
-    const long long left = t.n - base;
-    const int n = left >= 8 ? 8 : (left > 0 ? (int)left : 0);
-    const int full = n == 8 ? t.vec : 0;
+// one thread's elements of one chunk, as loaded.  MASTER: the parameter's value
+// is its 32-bit copy
+template <class T, int BITS, bool MASTER>
+struct Chunk {
+    using P = typename std::conditional<MASTER, float, T>::type;
+    long long base;
+    int n, vec;
+    Raw8<T> g;
+    Raw8<P> p;
+    Raw8<float> m, v;   // BITS 32
+    uint2 mc, vc;       // BITS 8
+    uint8_t ms, vs;
+
+    __device__ __forceinline__ void load(const OptTensor& t, long long at) {
+        base = at;
+        const long long left = t.n - base;
+        n = left >= 8 ? 8 : (left > 0 ? (int)left : 0);
+        vec = n == 8 ? t.vec : 0;
+        load8(static_cast<const T*>(t.g) + base, vec, n, g);
+        load8((MASTER ? reinterpret_cast<const P*>(t.master) : static_cast<const P*>(t.p)) + base,
+              vec, n, p);
+        if constexpr (BITS == 8) {
+            mc = load_codes(static_cast<const uint8_t*>(t.m) + base, vec, n);
+            vc = load_codes(static_cast<const uint8_t*>(t.v) + base, vec, n);
+            // a lane behind the tensor's end may be behind the scales' end too
+            ms = n > 0 ? t.ms[base / kOptBlock] : 1;
+            vs = n > 0 ? t.vs[base / kOptBlock] : 1;
+        } else {
+            load8(static_cast<const float*>(t.m) + base, vec, n, m);
+            load8(static_cast<const float*>(t.v) + base, vec, n, v);
+        }
+    }
+};
+
+template <class T, int BITS, bool MASTER>
+__device__ __forceinline__ void update8(const OptTensor& t, const Chunk<T, BITS, MASTER>& c,
+                                        const OptArgs& a, const StepScalars& s, unsigned key) {
+    const long long base = c.base;
+    const int n = c.n, vec = c.vec;
     float g[8], p[8], m[8], v[8];
-    load8(static_cast<const T*>(t.g) + base, full, n, g);
-    if (t.master) load8(t.master + base, full, n, p);
-    else load8(static_cast<const T*>(t.p) + base, full, n, p);
-    const long long block = base / kOptBlock;
+    unpack(c.g, g);
+    unpack(c.p, p);
     if constexpr (BITS == 8) {
-        const uint2 mc = load_codes(static_cast<const uint8_t*>(t.m) + base, full, n);
-        const uint2 vc = load_codes(static_cast<const uint8_t*>(t.v) + base, full, n);
-        // a lane behind the tensor's end may be behind the scales' end too.
-        // The scales are powers of two: b (code s) = code (b s)
-        const float ms = scale_of(n > 0 ? t.ms[block] : 1), vs = scale_of(n > 0 ? t.vs[block] : 1);
-        decode8<__NV_E4M3>(mc, __fmul_rn(ms, a.b1), m);
-        decode8<__NV_E5M2>(vc, __fmul_rn(vs, a.b2), v);
+        // the scales are powers of two: b (code s) = code (b s)
+        decode8<__NV_E4M3>(c.mc, __fmul_rn(scale_of(c.ms), a.b1), m);
+        decode8<__NV_E5M2>(c.vc, __fmul_rn(scale_of(c.vs), a.b2), v);
     } else {
-        load8(static_cast<const float*>(t.m) + base, full, n, m);
-        load8(static_cast<const float*>(t.v) + base, full, n, v);
+        unpack(c.m, m);
+        unpack(c.v, v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             m[i] = __fmul_rn(m[i], a.b1);
@@ -280,22 +360,23 @@ __device__ __forceinline__ void update8(const OptTensor& t, long long base, cons
         m[i] = __fadd_rn(m[i], __fmul_rn(gi, a.omb1));
         v[i] = __fadd_rn(v[i], __fmul_rn(__fmul_rn(gi, gi), a.omb2));
         // root and quotient to 2^-22: their last bits are far below the
-        // update's own, and correctly rounded ones take half of the instructions
-        const float d = __fadd_rn(__fmul_rn(sqrt_approx(v[i]), s.root), a.eps);
-        p[i] = __fsub_rn(__fmul_rn(p[i], s.decay), __fmul_rn(__fdividef(m[i], d), s.rate));
+        // parameter's own, and correctly rounded ones took a third of all
+        // instructions.  A v below 2^-126 counts as 2^-126 here.
+        const float d = __fadd_rn(__fmul_rn(root_of(v[i]), s.root), a.eps);
+        p[i] = __fsub_rn(__fmul_rn(p[i], s.decay), __fmul_rn(quotient(m[i], d), s.rate));
     }
-    if (t.master) store8(t.master + base, full, n, p);
-    store8(static_cast<T*>(t.p) + base, full, n, p);
+    if constexpr (MASTER) store8(t.master + base, vec, n, p);
+    store8(static_cast<T*>(t.p) + base, vec, n, p);
     if constexpr (BITS == 8) {
         // elements behind the end are zeros: they change no maximum
-        unsigned mtop = 0, vtop = 0;
+        float mmax = fabsf(m[0]), vmax = v[0];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            mtop = max(mtop, __float_as_uint(m[i]) & 0x7fffffffu);
-            vtop = max(vtop, __float_as_uint(v[i]) & 0x7fffffffu);
+        for (int i = 1; i < 8; ++i) {
+            mmax = max_nan(mmax, fabsf(m[i]));
+            vmax = max_nan(vmax, v[i]);
         }
-        mtop = __reduce_max_sync(0xffffffffu, mtop);
-        vtop = __reduce_max_sync(0xffffffffu, vtop);
+        const unsigned mtop = __reduce_max_sync(0xffffffffu, __float_as_uint(mmax));
+        const unsigned vtop = __reduce_max_sync(0xffffffffu, __float_as_uint(vmax));
         uint2 mc, vc;
         int mk, vk;
         // above 1.75 * 2^127 the scales are the largest (or there is none)
@@ -303,15 +384,15 @@ __device__ __forceinline__ void update8(const OptTensor& t, long long base, cons
             encode_moments<true>(m, v, n, mtop, vtop, (unsigned)base, key, mc, vc, mk, vk);
         else
             encode_moments<false>(m, v, n, mtop, vtop, (unsigned)base, key, mc, vc, mk, vk);
-        store_codes(static_cast<uint8_t*>(t.m) + base, full, n, mc);
-        store_codes(static_cast<uint8_t*>(t.v) + base, full, n, vc);
+        store_codes(static_cast<uint8_t*>(t.m) + base, vec, n, mc);
+        store_codes(static_cast<uint8_t*>(t.v) + base, vec, n, vc);
         if ((threadIdx.x & 31) == 0 && n > 0) {
-            t.ms[block] = (uint8_t)mk;
-            t.vs[block] = (uint8_t)vk;
+            t.ms[base / kOptBlock] = (uint8_t)mk;
+            t.vs[base / kOptBlock] = (uint8_t)vk;
         }
     } else {
-        store8(static_cast<float*>(t.m) + base, full, n, m);
-        store8(static_cast<float*>(t.v) + base, full, n, v);
+        store8(static_cast<float*>(t.m) + base, vec, n, m);
+        store8(static_cast<float*>(t.v) + base, vec, n, v);
     }
 }
 
@@ -333,10 +414,16 @@ struct ChunkPlan {
     unsigned key;
 };
 
-template <int N, int BITS>
+template <int N, class T, int BITS, bool MASTER>
 __global__ void __launch_bounds__(kThreads)
 adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ OptArgs a) {
     __shared__ ChunkPlan plan[kThreads];
+    // the CTA's chunks are one grid apart (neighbouring CTAs share DRAM pages);
+    // the next one is on its way while one is computed
+    Chunk<T, BITS, MASTER> here;
+    const int first = find_tensor(tab, blockIdx.x);
+    const long long lane = threadIdx.x * kLane;
+    here.load(tab.t[first], (long long)(blockIdx.x - tab.t[first].chunk0) * kChunk + lane);
     const double lr = a.lr_dev ? (double)*a.lr_dev : a.lr;
     StepScalars s{};
     s.decay = (float)(1.0 - lr * a.wd);
@@ -345,11 +432,11 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
         const double c = a.max_norm / (*a.norm + 1e-6);
         s.clip = c > 1.0 ? 1.f : (float)c;   // NaN stays NaN
     }
-    // the CTA's chunks are one grid apart (neighbouring CTAs share DRAM pages).
-    // What each of them needs of its tensor -- which one it is, powers of the
-    // betas in 64 bits -- is worked out by one thread a chunk, a CTA's width of
-    // chunks at a time
-    for (unsigned c0 = blockIdx.x; c0 < tab.chunks; c0 += kThreads * gridDim.x) {
+    // What a chunk needs of its tensor -- which one it is, powers of the betas in
+    // 64 bits -- is worked out by one thread a chunk, a CTA's width of chunks at
+    // a time (and the first one again as the next width's)
+    constexpr unsigned kWidth = kThreads - 1;
+    for (unsigned c0 = blockIdx.x; c0 < tab.chunks; c0 += kWidth * gridDim.x) {
         __syncthreads();
         const unsigned long long mine = c0 + (unsigned long long)threadIdx.x * gridDim.x;
         if (mine < tab.chunks) {
@@ -364,16 +451,18 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
         }
         __syncthreads();
         unsigned c = c0;
-        for (int k = 0; k < kThreads && c < tab.chunks; ++k, c += gridDim.x) {
+        for (unsigned k = 0; k < kWidth && c < tab.chunks; ++k, c += gridDim.x) {
             const ChunkPlan q = plan[k];
-            const OptTensor& t = tab.t[q.tensor];
-            const long long base = (long long)(c - t.chunk0) * kChunk + threadIdx.x * kLane;
+            Chunk<T, BITS, MASTER> next;
+            if (c + gridDim.x < tab.chunks) {
+                const OptTensor& u = tab.t[plan[k + 1].tensor];
+                next.load(u, (long long)(c + gridDim.x - u.chunk0) * kChunk + lane);
+            }
             s.rate = q.rate;
             s.root = q.root;
-            const unsigned key = BITS == 8 ? mix32(q.key + (unsigned)(base >> 32)) : 0;
-            if (t.dtype == kOptF32) update8<float, BITS>(t, base, a, s, key);
-            else if (t.dtype == kOptBf16) update8<__nv_bfloat16, BITS>(t, base, a, s, key);
-            else update8<__half, BITS>(t, base, a, s, key);
+            const unsigned key = BITS == 8 ? mix32(q.key + (unsigned)(here.base >> 32)) : 0;
+            update8(tab.t[q.tensor], here, a, s, key);
+            here = next;
         }
     }
     // every CTA has read the counts it needs: the last one to come here
@@ -394,8 +483,10 @@ __device__ __forceinline__ void squares8(const T* p, long long base, long long s
                                          double (&sum)[4]) {
     const long long left = size - base;
     const int n = left >= 8 ? 8 : (left > 0 ? (int)left : 0);
+    Raw8<T> r;
     float x[8];
-    load8(p + base, n == 8 ? vec : 0, n, x);
+    load8(p + base, n == 8 ? vec : 0, n, r);
+    unpack(r, x);
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum[i & 3] = fma((double)x[i], (double)x[i], sum[i & 3]);
 }
@@ -457,7 +548,7 @@ norm_kernel(const __grid_constant__ OptTable<N> tab, double* partial, int first,
     }
 }
 
-// CTAs of one launch: all chunks at once up to what the SMs hold, then a loop
+// CTAs of one launch: one a chunk, up to what the SMs hold at a time
 unsigned opt_grid(unsigned chunks, unsigned most) {
     return chunks < 1 ? 1 : (chunks < most ? chunks : most);
 }
@@ -474,14 +565,43 @@ void fill(OptTable<N>* tab, const OptTensor* t, int count) {
     tab->chunks = c;
 }
 
-template <int N>
+// CTAs of a kernel that the GPU holds at a time (asked once)
+template <class K>
+unsigned resident_ctas(K kernel) {
+    int device = 0, sms = 148, per_sm = 1;
+    if (cudaGetDevice(&device) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, 0) != cudaSuccess ||
+        per_sm < 1) {
+        cudaGetLastError();
+        return 148;
+    }
+    return (unsigned)(sms * per_sm);
+}
+
+template <int N, class T, int BITS, bool MASTER>
+cudaError_t adamw_launch(const OptTable<N>& tab, const OptArgs& a, cudaStream_t s) {
+    static const unsigned most = resident_ctas(adamw_kernel<N, T, BITS, MASTER>);
+    adamw_kernel<N, T, BITS, MASTER><<<opt_grid(tab.chunks, most), kThreads, 0, s>>>(tab, a);
+    return cudaGetLastError();
+}
+
+template <int N, class T, bool MASTER>
 cudaError_t adamw_part(const OptTensor* t, int count, int bits, const OptArgs& a, cudaStream_t s) {
     OptTable<N> tab;
     fill(&tab, t, count);
-    const unsigned grid = opt_grid(tab.chunks, kOptCtas);
-    if (bits == 8) adamw_kernel<N, 8><<<grid, kThreads, 0, s>>>(tab, a);
-    else adamw_kernel<N, 32><<<grid, kThreads, 0, s>>>(tab, a);
-    return cudaGetLastError();
+    return bits == 8 ? adamw_launch<N, T, 8, MASTER>(tab, a, s)
+                     : adamw_launch<N, T, 32, MASTER>(tab, a, s);
+}
+
+template <int N>
+cudaError_t adamw_typed(const OptTensor* t, int count, int bits, const OptArgs& a, cudaStream_t s) {
+    if (t->dtype == kOptF32) return adamw_part<N, float, false>(t, count, bits, a, s);
+    if (t->dtype == kOptBf16)
+        return t->master ? adamw_part<N, __nv_bfloat16, true>(t, count, bits, a, s)
+                         : adamw_part<N, __nv_bfloat16, false>(t, count, bits, a, s);
+    return t->master ? adamw_part<N, __half, true>(t, count, bits, a, s)
+                     : adamw_part<N, __half, false>(t, count, bits, a, s);
 }
 
 template <int N>
@@ -504,9 +624,9 @@ constexpr int kSmall = 12, kMiddle = 100;
 
 cudaError_t launch_adamw(const OptTensor* t, int count, int bits, OptArgs a, cudaStream_t s) {
     a.seed_key = mix32(a.seed_key);
-    if (count <= kSmall) return adamw_part<kSmall>(t, count, bits, a, s);
-    if (count <= kMiddle) return adamw_part<kMiddle>(t, count, bits, a, s);
-    return adamw_part<kOptTensors>(t, count, bits, a, s);
+    if (count <= kSmall) return adamw_typed<kSmall>(t, count, bits, a, s);
+    if (count <= kMiddle) return adamw_typed<kMiddle>(t, count, bits, a, s);
+    return adamw_typed<kOptTensors>(t, count, bits, a, s);
 }
 
 cudaError_t launch_grad_norm(const OptTensor* t, int count, double* partial, int* first, bool last,
