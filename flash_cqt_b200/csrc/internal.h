@@ -272,13 +272,15 @@ struct OptTensor {
 };
 
 struct OptArgs {
-    double lr, wd, lb1, lb2;   // lb: log2 of the betas
+    double lr, wd;
     const float* lr_dev;       // not null: the rate is read from the device
     const double* norm;        // not null: gradients are scaled to max_norm
     double max_norm;
     unsigned* ticket;          // zero between launches
     float b1, omb1, b2, omb2, eps;
+    float ln1, ln2;            // logarithms of the betas
     unsigned seed_key;
+    unsigned two20, two21;     // 2^20 and 2^21, not known when the kernel is compiled
 };
 
 // one launch over 1 to kOptTensors tensors of one type, all with a master copy

@@ -60,10 +60,15 @@ __host__ __device__ __forceinline__ unsigned mix32(unsigned x) {
     return x ^ (x >> 16);
 }
 
-// the larger of two, NaN if either is
-__device__ __forceinline__ float max_nan(float a, float b) {
+// the largest of three, NaN if one of them is
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
     float y;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+__device__ __forceinline__ unsigned mad_hi(unsigned a, unsigned b, unsigned c) {
+    unsigned y;
+    asm("mad.hi.u32 %0, %1, %2, %3;" : "=r"(y) : "r"(a), "r"(b), "r"(c));
     return y;
 }
 
@@ -182,10 +187,10 @@ __device__ __forceinline__ void store_codes(uint8_t* p, int vec, int n, uint2 c)
             if (i < n) p[i] = (uint8_t)((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
     }
 }
-// sqrt(max(x, 2^-126)) and a / b to 2^-22
+// sqrt(x + 2^-126) and a / b to 2^-22
 __device__ __forceinline__ float root_of(float x) {
     float y;
-    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(max_nan(x, 0x1p-126f)));
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(__fadd_rn(x, 0x1p-126f)));
     return y;
 }
 __device__ __forceinline__ float quotient(float a, float b) {
@@ -224,8 +229,7 @@ __device__ __forceinline__ float scale_of(uint8_t byte) {
     return __uint_as_float(byte ? (unsigned)byte << 23 : 0x400000u);
 }
 
-// what one step needs of one tensor's count: lr / (1 - b1^t), 1 / sqrt(1 -
-// b2^t), in 64 bits up to the last rounding
+// 1 - lr wd, lr / (1 - b1^t), 1 / sqrt(1 - b2^t) and the gradients' factor
 struct StepScalars {
     float decay, rate, root, clip;
 };
@@ -244,8 +248,8 @@ struct StepScalars {
 template <bool RARE>
 __device__ __forceinline__ void encode_moments(const float (&m)[8], const float (&v)[8], int n,
                                                unsigned mtop, unsigned vtop, unsigned index,
-                                               unsigned key, uint2& mc, uint2& vc, int& mk,
-                                               int& vk) {
+                                               unsigned key, const OptArgs& k, uint2& mc,
+                                               uint2& vc, int& mk, int& vk) {
     if constexpr (RARE) {
         mtop = vtop = 0;
 #pragma unroll
@@ -271,11 +275,15 @@ __device__ __forceinline__ void encode_moments(const float (&m)[8], const float 
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const unsigned h = mix_middle(first ^ i);
-        // the low and the high half of mix32's result (its last step folds the
-        // high half into the low one)
-        const unsigned hm = ((h << 4) ^ (h >> 12)) & 0xffff0u, hv = (h >> 11) & 0x1fffe0u;
-        const unsigned mb = __float_as_uint(__fmul_rn(m[i], mi)) + hm + 8u;
-        const unsigned vb = __float_as_uint(__fmul_rn(v[i], vi)) + hv + 16u;
+        // hm and hv: the low and the high half of mix32's result (its last step
+        // folds the high half into the low one) in the upper 16 bits, and half a
+        // step below.  The high half of a product with 2^20 (2^21) is that
+        // shifted to where the noise goes; it runs beside the integer adders
+        // and shifters, which are what this kernel has least of.
+        const unsigned hm = (((h << 16) ^ h) & 0xffff0000u) | 0x8000u;
+        const unsigned hv = (h & 0xffff0000u) | 0x8000u;
+        const unsigned mb = mad_hi(hm, k.two20, __float_as_uint(__fmul_rn(m[i], mi)));
+        const unsigned vb = mad_hi(hv, k.two21, __float_as_uint(__fmul_rn(v[i], vi)));
         a[i] = __uint_as_float(mb & 0xfff00000u);
         b[i] = __uint_as_float(vb & 0xffe00000u);
         if constexpr (RARE) {
@@ -283,9 +291,11 @@ __device__ __forceinline__ void encode_moments(const float (&m)[8], const float 
             a[i] = fminf(fmaxf(a[i], -mmost), mmost);
             b[i] = fminf(b[i], vmost);
         }
-        // below the smallest normal value: 0 for m, that value for v
-        if (!(fabsf(a[i]) >= 0x1p-6f)) a[i] = 0.f;
-        b[i] = v[i] > 0.f ? fmaxf(b[i], 0x1p-14f) : 0.f;
+        // below the smallest normal value: 0 for m, that value for v.  |a| is at
+        // most 1.875 * 2^-7 or at least 2^-6, its square 0.88 * 2^-12 or 2^-12:
+        // a factor of 0 or 1, again beside the adders
+        a[i] = __fmul_rn(a[i], __saturatef(fmaf(__fmul_rn(a[i], a[i]), 0x1p40f, -0.94f * 0x1p28f)));
+        b[i] = fmaxf(b[i], fminf(__fmul_rn(__fmul_rn(v[i], 0x1p100f), 0x1p100f), 0x1p-14f));
     }
     mc = to_fp8<__NV_E4M3>(a);
     vc = to_fp8<__NV_E5M2>(b);
@@ -305,18 +315,14 @@ template <class T, int BITS, bool MASTER>
 struct Chunk {
     using P = typename std::conditional<MASTER, float, T>::type;
     long long base;
-    int n, vec;
     Raw8<T> g;
     Raw8<P> p;
     Raw8<float> m, v;   // BITS 32
     uint2 mc, vc;       // BITS 8
     uint8_t ms, vs;
 
-    __device__ __forceinline__ void load(const OptTensor& t, long long at) {
+    __device__ __forceinline__ void load(const OptTensor& t, long long at, int n, int vec) {
         base = at;
-        const long long left = t.n - base;
-        n = left >= 8 ? 8 : (left > 0 ? (int)left : 0);
-        vec = n == 8 ? t.vec : 0;
         load8(static_cast<const T*>(t.g) + base, vec, n, g);
         load8((MASTER ? reinterpret_cast<const P*>(t.master) : static_cast<const P*>(t.p)) + base,
               vec, n, p);
@@ -335,9 +341,8 @@ struct Chunk {
 
 template <class T, int BITS, bool MASTER>
 __device__ __forceinline__ void update8(const OptTensor& t, const Chunk<T, BITS, MASTER>& c,
-                                        const OptArgs& a, const StepScalars& s, unsigned key) {
-    const long long base = c.base;
-    const int n = c.n, vec = c.vec;
+                                        const OptArgs& a, const StepScalars& s, unsigned key,
+                                        int n, int vec) {
     float g[8], p[8], m[8], v[8];
     unpack(c.g, g);
     unpack(c.p, p);
@@ -361,39 +366,55 @@ __device__ __forceinline__ void update8(const OptTensor& t, const Chunk<T, BITS,
         v[i] = __fadd_rn(v[i], __fmul_rn(__fmul_rn(gi, gi), a.omb2));
         // root and quotient to 2^-22: their last bits are far below the
         // parameter's own, and correctly rounded ones took a third of all
-        // instructions.  A v below 2^-126 counts as 2^-126 here.
+        // instructions.  2^-126 under the root keeps what is subnormal
+        // from being read as 0 (above 2^-102 it changes nothing).
         const float d = __fadd_rn(__fmul_rn(root_of(v[i]), s.root), a.eps);
         p[i] = __fsub_rn(__fmul_rn(p[i], s.decay), __fmul_rn(quotient(m[i], d), s.rate));
     }
-    if constexpr (MASTER) store8(t.master + base, vec, n, p);
-    store8(static_cast<T*>(t.p) + base, vec, n, p);
+    uint2 mc, vc;
+    int mk, vk;
     if constexpr (BITS == 8) {
         // elements behind the end are zeros: they change no maximum
-        float mmax = fabsf(m[0]), vmax = v[0];
+        float mmax = 0.f, vmax = 0.f;
 #pragma unroll
-        for (int i = 1; i < 8; ++i) {
-            mmax = max_nan(mmax, fabsf(m[i]));
-            vmax = max_nan(vmax, v[i]);
+        for (int i = 0; i < 8; i += 2) {
+            mmax = max_nan(mmax, fabsf(m[i]), fabsf(m[i + 1]));
+            vmax = max_nan(vmax, v[i], v[i + 1]);
         }
         const unsigned mtop = __reduce_max_sync(0xffffffffu, __float_as_uint(mmax));
         const unsigned vtop = __reduce_max_sync(0xffffffffu, __float_as_uint(vmax));
-        uint2 mc, vc;
-        int mk, vk;
         // above 1.75 * 2^127 the scales are the largest (or there is none)
         if (max(mtop, vtop) > 0x7f600000u)
-            encode_moments<true>(m, v, n, mtop, vtop, (unsigned)base, key, mc, vc, mk, vk);
+            encode_moments<true>(m, v, n, mtop, vtop, (unsigned)c.base, key, a, mc, vc, mk, vk);
         else
-            encode_moments<false>(m, v, n, mtop, vtop, (unsigned)base, key, mc, vc, mk, vk);
-        store_codes(static_cast<uint8_t*>(t.m) + base, vec, n, mc);
-        store_codes(static_cast<uint8_t*>(t.v) + base, vec, n, vc);
+            encode_moments<false>(m, v, n, mtop, vtop, (unsigned)c.base, key, a, mc, vc, mk, vk);
+    }
+    if constexpr (MASTER) store8(t.master + c.base, vec, n, p);
+    store8(static_cast<T*>(t.p) + c.base, vec, n, p);
+    if constexpr (BITS == 8) {
+        store_codes(static_cast<uint8_t*>(t.m) + c.base, vec, n, mc);
+        store_codes(static_cast<uint8_t*>(t.v) + c.base, vec, n, vc);
         if ((threadIdx.x & 31) == 0 && n > 0) {
-            t.ms[base / kOptBlock] = (uint8_t)mk;
-            t.vs[base / kOptBlock] = (uint8_t)vk;
+            t.ms[c.base / kOptBlock] = (uint8_t)mk;
+            t.vs[c.base / kOptBlock] = (uint8_t)vk;
         }
     } else {
-        store8(static_cast<float*>(t.m) + base, vec, n, m);
-        store8(static_cast<float*>(t.v) + base, vec, n, v);
+        store8(static_cast<float*>(t.m) + c.base, vec, n, m);
+        store8(static_cast<float*>(t.v) + c.base, vec, n, v);
     }
+}
+
+// a chunk that ends inside the tensor's last 8 * kThreads elements or whose
+// arrays are not aligned
+template <class T, int BITS, bool MASTER>
+__device__ __forceinline__ void update_part(const OptTensor& t, long long base, const OptArgs& a,
+                                         const StepScalars& s, unsigned key) {
+    const long long left = t.n - base;
+    const int n = left >= 8 ? 8 : (left > 0 ? (int)left : 0);
+    const int vec = n == 8 ? t.vec : 0;
+    Chunk<T, BITS, MASTER> c;
+    c.load(t, base, n, vec);
+    update8(t, c, a, s, key, n, vec);
 }
 
 // the tensor that chunk c lies in: the last one whose first chunk is <= c
@@ -408,71 +429,97 @@ __device__ __forceinline__ int find_tensor(const OptTable<N>& tab, unsigned c) {
     return lo;
 }
 
-struct ChunkPlan {
-    int tensor;
+constexpr int kWhole = 1 << 30;   // every thread has 8 aligned elements
+
+// whether chunk c of the tensor has all its elements, aligned
+__device__ __forceinline__ bool is_whole(const OptTensor& t, unsigned c) {
+    return t.vec == 2 && (long long)(c - t.chunk0 + 1) * kChunk <= t.n;
+}
+
+struct TensorPlan {
     float rate, root;
     unsigned key;
+    unsigned chunk0;
 };
 
 template <int N, class T, int BITS, bool MASTER>
 __global__ void __launch_bounds__(kThreads)
 adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ OptArgs a) {
-    __shared__ ChunkPlan plan[kThreads];
-    // the CTA's chunks are one grid apart (neighbouring CTAs share DRAM pages);
-    // the next one is on its way while one is computed
+    __shared__ TensorPlan tensor[N];
+    __shared__ int chunk[kThreads];      // tensor of each of the CTA's next chunks, and kWhole
+    __shared__ long long steps[N];
+    __shared__ StepScalars same;
+    __shared__ unsigned order;
+    // The CTA's chunks are one grid apart (neighbouring CTAs share DRAM pages).
+    // The next one is on its way while one is computed, and the first one while
+    // what follows works out the scalars.
     Chunk<T, BITS, MASTER> here;
-    const int first = find_tensor(tab, blockIdx.x);
     const long long lane = threadIdx.x * kLane;
-    here.load(tab.t[first], (long long)(blockIdx.x - tab.t[first].chunk0) * kChunk + lane);
-    const double lr = a.lr_dev ? (double)*a.lr_dev : a.lr;
-    StepScalars s{};
-    s.decay = (float)(1.0 - lr * a.wd);
-    s.clip = 1.f;
-    if (a.norm) {
-        const double c = a.max_norm / (*a.norm + 1e-6);
-        s.clip = c > 1.0 ? 1.f : (float)c;   // NaN stays NaN
+    const int first = find_tensor(tab, blockIdx.x);
+    if (is_whole(tab.t[first], blockIdx.x))
+        here.load(tab.t[first], (long long)(blockIdx.x - tab.t[first].chunk0) * kChunk + lane, 8, 2);
+    if (threadIdx.x == kThreads - 1) {
+        same.decay = (float)(1.0 - (a.lr_dev ? (double)*a.lr_dev : a.lr) * a.wd);
+        const double c = a.norm ? a.max_norm / (*a.norm + 1e-6) : 1.0;
+        same.clip = c > 1.0 ? 1.f : (float)c;   // NaN stays NaN
     }
-    // What a chunk needs of its tensor -- which one it is, powers of the betas in
-    // 64 bits -- is worked out by one thread a chunk, a CTA's width of chunks at
-    // a time (and the first one again as the next width's)
+    // 1 - b^t = -expm1(t ln b), which 32 bits hold to 2^-22 for every t
+    const float lr = a.lr_dev ? *a.lr_dev : (float)a.lr;
+    for (int i = threadIdx.x; i < tab.count; i += kThreads) {
+        const OptTensor& t = tab.t[i];
+        const long long step = *t.step + 1;
+        TensorPlan q;
+        q.rate = lr / -expm1f((float)step * a.ln1);
+        q.root = rsqrtf(-expm1f((float)step * a.ln2));
+        q.key = BITS == 8 ? mix32(mix32(a.seed_key + (unsigned)step) + (unsigned)t.ordinal) : 0;
+        q.chunk0 = t.chunk0;
+        tensor[i] = q;
+        steps[i] = step;
+    }
+    // tensors are looked up by one thread a chunk, a CTA's width at a time (the
+    // last of a width is the first of the next)
     constexpr unsigned kWidth = kThreads - 1;
     for (unsigned c0 = blockIdx.x; c0 < tab.chunks; c0 += kWidth * gridDim.x) {
         __syncthreads();
         const unsigned long long mine = c0 + (unsigned long long)threadIdx.x * gridDim.x;
         if (mine < tab.chunks) {
-            ChunkPlan q;
-            q.tensor = find_tensor(tab, (unsigned)mine);
-            const OptTensor& t = tab.t[q.tensor];
-            const long long step = *t.step + 1;
-            q.rate = (float)(lr / (1.0 - exp2((double)step * a.lb1)));
-            q.root = (float)(1.0 / sqrt(1.0 - exp2((double)step * a.lb2)));
-            q.key = BITS == 8 ? mix32(mix32(a.seed_key + (unsigned)step) + (unsigned)t.ordinal) : 0;
-            plan[threadIdx.x] = q;
+            int lo = 0, hi = tab.count - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (tensor[mid].chunk0 <= (unsigned)mine) lo = mid;
+                else hi = mid - 1;
+            }
+            chunk[threadIdx.x] = lo | (is_whole(tab.t[lo], (unsigned)mine) ? kWhole : 0);
         }
         __syncthreads();
+        StepScalars s = same;
         unsigned c = c0;
         for (unsigned k = 0; k < kWidth && c < tab.chunks; ++k, c += gridDim.x) {
-            const ChunkPlan q = plan[k];
-            Chunk<T, BITS, MASTER> next;
-            if (c + gridDim.x < tab.chunks) {
-                const OptTensor& u = tab.t[plan[k + 1].tensor];
-                next.load(u, (long long)(c + gridDim.x - u.chunk0) * kChunk + lane);
-            }
+            const int i = chunk[k];
+            const OptTensor& t = tab.t[i & ~kWhole];
+            const TensorPlan q = tensor[i & ~kWhole];
             s.rate = q.rate;
             s.root = q.root;
-            const unsigned key = BITS == 8 ? mix32(q.key + (unsigned)(here.base >> 32)) : 0;
-            update8(tab.t[q.tensor], here, a, s, key);
+            const bool more = c + gridDim.x < tab.chunks;
+            const int j = more ? chunk[k + 1] : 0;
+            Chunk<T, BITS, MASTER> next;
+            if (j & kWhole) {
+                const OptTensor& u = tab.t[j & ~kWhole];
+                next.load(u, (long long)(c + gridDim.x - u.chunk0) * kChunk + lane, 8, 2);
+            }
+            const long long base = (long long)(c - q.chunk0) * kChunk + lane;
+            const unsigned key = BITS == 8 ? mix32(q.key + (unsigned)(base >> 32)) : 0;
+            if (i & kWhole) update8(t, here, a, s, key, 8, 2);
+            else update_part<T, BITS, MASTER>(t, base, a, s, key);
             here = next;
         }
     }
-    // every CTA has read the counts it needs: the last one to come here
-    // advances them
-    __shared__ unsigned order;
+    // every CTA has read the counts: the last one to come here advances them
     __syncthreads();
     if (threadIdx.x == 0) order = atomicAdd(a.ticket, 1u);
     __syncthreads();
     if (order != gridDim.x - 1) return;
-    for (int i = threadIdx.x; i < tab.count; i += kThreads) *tab.t[i].step += 1;
+    for (int i = threadIdx.x; i < tab.count; i += kThreads) *tab.t[i].step = steps[i];
     if (threadIdx.x == 0) *a.ticket = 0;
 }
 
@@ -624,6 +671,8 @@ constexpr int kSmall = 12, kMiddle = 100;
 
 cudaError_t launch_adamw(const OptTensor* t, int count, int bits, OptArgs a, cudaStream_t s) {
     a.seed_key = mix32(a.seed_key);
+    a.two20 = 1u << 20;
+    a.two21 = 1u << 21;
     if (count <= kSmall) return adamw_typed<kSmall>(t, count, bits, a, s);
     if (count <= kMiddle) return adamw_typed<kMiddle>(t, count, bits, a, s);
     return adamw_typed<kOptTensors>(t, count, bits, a, s);
