@@ -35,10 +35,19 @@ namespace fcqt {
 
 namespace {
 
-constexpr int kThreads = 256;
 constexpr int kLane = 8;                        // consecutive elements a thread
-constexpr int kChunk = kThreads * kLane;        // elements a CTA takes at a time
-static_assert(kChunk % kOptBlock == 0 && 32 * kLane == kOptBlock, "a warp is one block");
+static_assert(32 * kLane == kOptBlock, "a warp is one block");
+// CTA sizes.  The step: 28 warps an SM with 72 registers for 8-bit moments, 16
+// with 128 for 32-bit ones, which move more bytes an element.  Measured, 67 M
+// float elements with 8-bit moments: 174 us with 4 CTAs of 224 threads an SM
+// (172 with 2 of 448), 211 with 3 of 256, 225 with 4 of 192, 239 with 5 of 192;
+// 32-bit moments of 144 M bf16 elements: 660 us with 16 warps an SM, 675 with
+// 24, 750 with 32: what more loads in flight win they lose in DRAM pages.
+template <int BITS>
+constexpr int kStepThreads = BITS == 8 ? 224 : 256;
+template <int BITS>
+constexpr int kStepCtas = BITS == 8 ? 4 : 2;    // of an SM
+constexpr int kNormThreads = 256;
 
 template <int N>
 struct OptTable {
@@ -389,6 +398,8 @@ __device__ __forceinline__ void update8(const OptTensor& t, const Chunk<T, BITS,
         else
             encode_moments<false>(m, v, n, mtop, vtop, (unsigned)c.base, key, a, mc, vc, mk, vk);
     }
+    // all stores together: the parameter's ahead of the moments' rounding made
+    // 67 M elements take 229 us instead of 174
     if constexpr (MASTER) store8(t.master + c.base, vec, n, p);
     store8(static_cast<T*>(t.p) + c.base, vec, n, p);
     if constexpr (BITS == 8) {
@@ -404,8 +415,7 @@ __device__ __forceinline__ void update8(const OptTensor& t, const Chunk<T, BITS,
     }
 }
 
-// a chunk that ends inside the tensor's last 8 * kThreads elements or whose
-// arrays are not aligned
+// a chunk that the tensor ends in, or whose arrays are not aligned
 template <class T, int BITS, bool MASTER>
 __device__ __forceinline__ void update_part(const OptTensor& t, long long base, const OptArgs& a,
                                          const StepScalars& s, unsigned key) {
@@ -432,8 +442,9 @@ __device__ __forceinline__ int find_tensor(const OptTable<N>& tab, unsigned c) {
 constexpr int kWhole = 1 << 30;   // every thread has 8 aligned elements
 
 // whether chunk c of the tensor has all its elements, aligned
+template <int CHUNK>
 __device__ __forceinline__ bool is_whole(const OptTensor& t, unsigned c) {
-    return t.vec == 2 && (long long)(c - t.chunk0 + 1) * kChunk <= t.n;
+    return t.vec == 2 && (long long)(c - t.chunk0 + 1) * CHUNK <= t.n;
 }
 
 struct TensorPlan {
@@ -443,8 +454,9 @@ struct TensorPlan {
 };
 
 template <int N, class T, int BITS, bool MASTER>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kStepThreads<BITS>, kStepCtas<BITS>)
 adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ OptArgs a) {
+    constexpr int kThreads = kStepThreads<BITS>, kChunk = kThreads * kLane;
     __shared__ TensorPlan tensor[N];
     __shared__ int chunk[kThreads];      // tensor of each of the CTA's next chunks, and kWhole
     __shared__ long long steps[N];
@@ -456,7 +468,7 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
     Chunk<T, BITS, MASTER> here;
     const long long lane = threadIdx.x * kLane;
     const int first = find_tensor(tab, blockIdx.x);
-    if (is_whole(tab.t[first], blockIdx.x))
+    if (is_whole<kChunk>(tab.t[first], blockIdx.x))
         here.load(tab.t[first], (long long)(blockIdx.x - tab.t[first].chunk0) * kChunk + lane, 8, 2);
     if (threadIdx.x == kThreads - 1) {
         same.decay = (float)(1.0 - (a.lr_dev ? (double)*a.lr_dev : a.lr) * a.wd);
@@ -489,7 +501,7 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
                 if (tensor[mid].chunk0 <= (unsigned)mine) lo = mid;
                 else hi = mid - 1;
             }
-            chunk[threadIdx.x] = lo | (is_whole(tab.t[lo], (unsigned)mine) ? kWhole : 0);
+            chunk[threadIdx.x] = lo | (is_whole<kChunk>(tab.t[lo], (unsigned)mine) ? kWhole : 0);
         }
         __syncthreads();
         StepScalars s = same;
@@ -526,50 +538,98 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
 // ---- sqrt(sum of squares over all gradients), summed in 64 bits in a fixed
 // order: threads, warps, CTAs, launches
 template <class T>
-__device__ __forceinline__ void squares8(const T* p, long long base, long long size, int vec,
-                                         double (&sum)[4]) {
-    const long long left = size - base;
-    const int n = left >= 8 ? 8 : (left > 0 ? (int)left : 0);
-    Raw8<T> r;
+__device__ __forceinline__ void add_squares(const Raw8<T>& r, double (&sum)[4]) {
     float x[8];
-    load8(p + base, n == 8 ? vec : 0, n, r);
     unpack(r, x);
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum[i & 3] = fma((double)x[i], (double)x[i], sum[i & 3]);
 }
 
+// the chunk's 8 elements of a thread, some of them or none
+template <class T>
+__device__ __forceinline__ void squares8(const OptTensor& t, long long base, double (&sum)[4]) {
+    const long long left = t.n - base;
+    const int n = left >= 8 ? 8 : (left > 0 ? (int)left : 0);
+    Raw8<T> r;
+    load8(static_cast<const T*>(t.g) + base, n == 8 ? t.vec : 0, n, r);
+    add_squares(r, sum);
+}
+
 __device__ __forceinline__ double cta_sum(double x) {
-    __shared__ double part[kThreads / 32];
+    __shared__ double part[kNormThreads / 32];
 #pragma unroll
     for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) part[threadIdx.x / 32] = x;
     __syncthreads();
     x = 0;
-    for (int i = 0; i < kThreads / 32; ++i) x += part[i];
+    for (int i = 0; i < kNormThreads / 32; ++i) x += part[i];
     return x;
 }
 
 template <int N>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kNormThreads)
 norm_kernel(const __grid_constant__ OptTable<N> tab, double* partial, int first, int last,
             unsigned* ticket, double* norm, float* norm32) {
-    __shared__ int tensor[kThreads];   // of the CTA's next chunks, as above
+    constexpr int kChunk = kNormThreads * kLane;
+    __shared__ int tensor[kNormThreads];   // of each of the CTA's next chunks, and kWhole
     double part[4] = {0, 0, 0, 0};
-    for (unsigned c0 = blockIdx.x; c0 < tab.chunks; c0 += kThreads * gridDim.x) {
+    for (unsigned c0 = blockIdx.x; c0 < tab.chunks; c0 += kNormThreads * gridDim.x) {
         __syncthreads();
         const unsigned long long mine = c0 + (unsigned long long)threadIdx.x * gridDim.x;
-        if (mine < tab.chunks) tensor[threadIdx.x] = find_tensor(tab, (unsigned)mine);
+        if (mine < tab.chunks) {
+            const int i = find_tensor(tab, (unsigned)mine);
+            tensor[threadIdx.x] = i | (is_whole<kChunk>(tab.t[i], (unsigned)mine) ? kWhole : 0);
+        }
         __syncthreads();
+        // four chunks on their way at a time, where all of them are whole
+        constexpr unsigned kBatch = 4;
         unsigned c = c0;
-#pragma unroll 2
-        for (int k = 0; k < kThreads && c < tab.chunks; ++k, c += gridDim.x) {
-            const OptTensor& t = tab.t[tensor[k]];
-            const long long base = (long long)(c - t.chunk0) * kChunk + threadIdx.x * kLane;
-            if (t.dtype == kOptF32) squares8(static_cast<const float*>(t.g), base, t.n, t.vec, part);
-            else if (t.dtype == kOptBf16)
-                squares8(static_cast<const __nv_bfloat16*>(t.g), base, t.n, t.vec, part);
-            else squares8(static_cast<const __half*>(t.g), base, t.n, t.vec, part);
+        for (unsigned k = 0; k < kNormThreads && c < tab.chunks;) {
+            const bool all = k + kBatch <= kNormThreads &&
+                             c + (unsigned long long)(kBatch - 1) * gridDim.x < tab.chunks &&
+                             (tensor[k] & tensor[k + 1] & tensor[k + 2] & tensor[k + 3] & kWhole);
+            if (all) {
+                float4 r[kBatch][2];
+#pragma unroll
+                for (unsigned j = 0; j < kBatch; ++j) {
+                    const OptTensor& t = tab.t[tensor[k + j] & ~kWhole];
+                    const long long base =
+                        (long long)(c + j * gridDim.x - t.chunk0) * kChunk + threadIdx.x * kLane;
+                    if (t.dtype == kOptF32) {
+                        float x[8];
+                        load_v8(static_cast<const float*>(t.g) + base, x);
+                        r[j][0] = make_float4(x[0], x[1], x[2], x[3]);
+                        r[j][1] = make_float4(x[4], x[5], x[6], x[7]);
+                    } else {
+                        r[j][0] = *reinterpret_cast<const float4*>(
+                            static_cast<const unsigned short*>(t.g) + base);
+                    }
+                }
+#pragma unroll
+                for (unsigned j = 0; j < kBatch; ++j) {
+                    const int d = tab.t[tensor[k + j] & ~kWhole].dtype;
+                    if (d == kOptF32) {
+                        add_squares(Raw8<float>{{r[j][0].x, r[j][0].y, r[j][0].z, r[j][0].w,
+                                                 r[j][1].x, r[j][1].y, r[j][1].z, r[j][1].w}}, part);
+                    } else {
+                        const uint4 w = make_uint4(__float_as_uint(r[j][0].x), __float_as_uint(r[j][0].y),
+                                                   __float_as_uint(r[j][0].z), __float_as_uint(r[j][0].w));
+                        if (d == kOptBf16) add_squares(Raw8<__nv_bfloat16>{w}, part);
+                        else add_squares(Raw8<__half>{w}, part);
+                    }
+                }
+                k += kBatch;
+                c += kBatch * gridDim.x;
+            } else {
+                const OptTensor& t = tab.t[tensor[k] & ~kWhole];
+                const long long base = (long long)(c - t.chunk0) * kChunk + threadIdx.x * kLane;
+                if (t.dtype == kOptF32) squares8<float>(t, base, part);
+                else if (t.dtype == kOptBf16) squares8<__nv_bfloat16>(t, base, part);
+                else squares8<__half>(t, base, part);
+                ++k;
+                c += gridDim.x;
+            }
         }
     }
     double sum = (part[0] + part[1]) + (part[2] + part[3]);
@@ -587,7 +647,7 @@ norm_kernel(const __grid_constant__ OptTable<N> tab, double* partial, int first,
     if (!last) return;
     sum = 0;
     const int n = first + gridDim.x;
-    for (int i = threadIdx.x; i < n; i += kThreads) sum += __ldcg(partial + i);
+    for (int i = threadIdx.x; i < n; i += kNormThreads) sum += __ldcg(partial + i);
     sum = cta_sum(sum);
     if (threadIdx.x == 0) {
         *norm = sqrt(sum);
@@ -601,24 +661,24 @@ unsigned opt_grid(unsigned chunks, unsigned most) {
 }
 
 template <int N>
-void fill(OptTable<N>* tab, const OptTensor* t, int count) {
+void fill(OptTable<N>* tab, const OptTensor* t, int count, int chunk) {
     tab->count = count;
     unsigned c = 0;
     for (int i = 0; i < count; ++i) {
         tab->t[i] = t[i];
         tab->t[i].chunk0 = c;
-        c += (unsigned)((t[i].n + kChunk - 1) / kChunk);
+        c += (unsigned)((t[i].n + chunk - 1) / chunk);
     }
     tab->chunks = c;
 }
 
 // CTAs of a kernel that the GPU holds at a time (asked once)
 template <class K>
-unsigned resident_ctas(K kernel) {
+unsigned resident_ctas(K kernel, int threads) {
     int device = 0, sms = 148, per_sm = 1;
     if (cudaGetDevice(&device) != cudaSuccess ||
         cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, 0) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, 0) != cudaSuccess ||
         per_sm < 1) {
         cudaGetLastError();
         return 148;
@@ -627,18 +687,19 @@ unsigned resident_ctas(K kernel) {
 }
 
 template <int N, class T, int BITS, bool MASTER>
-cudaError_t adamw_launch(const OptTable<N>& tab, const OptArgs& a, cudaStream_t s) {
-    static const unsigned most = resident_ctas(adamw_kernel<N, T, BITS, MASTER>);
+cudaError_t adamw_launch(const OptTensor* t, int count, const OptArgs& a, cudaStream_t s) {
+    constexpr int kThreads = kStepThreads<BITS>;
+    OptTable<N> tab;
+    fill(&tab, t, count, kThreads * kLane);
+    static const unsigned most = resident_ctas(adamw_kernel<N, T, BITS, MASTER>, kThreads);
     adamw_kernel<N, T, BITS, MASTER><<<opt_grid(tab.chunks, most), kThreads, 0, s>>>(tab, a);
     return cudaGetLastError();
 }
 
 template <int N, class T, bool MASTER>
 cudaError_t adamw_part(const OptTensor* t, int count, int bits, const OptArgs& a, cudaStream_t s) {
-    OptTable<N> tab;
-    fill(&tab, t, count);
-    return bits == 8 ? adamw_launch<N, T, 8, MASTER>(tab, a, s)
-                     : adamw_launch<N, T, 32, MASTER>(tab, a, s);
+    return bits == 8 ? adamw_launch<N, T, 8, MASTER>(t, count, a, s)
+                     : adamw_launch<N, T, 32, MASTER>(t, count, a, s);
 }
 
 template <int N>
@@ -655,9 +716,9 @@ template <int N>
 cudaError_t norm_part(const OptTensor* t, int count, double* partial, int* first, bool last,
                       unsigned* ticket, double* norm, float* norm32, cudaStream_t s) {
     OptTable<N> tab;
-    fill(&tab, t, count);
+    fill(&tab, t, count, kNormThreads * kLane);
     const unsigned grid = opt_grid(tab.chunks, kNormCtas);
-    norm_kernel<N><<<grid, kThreads, 0, s>>>(tab, partial, *first, last ? 1 : 0, ticket, norm,
+    norm_kernel<N><<<grid, kNormThreads, 0, s>>>(tab, partial, *first, last ? 1 : 0, ticket, norm,
                                              norm32);
     *first += (int)grid;
     return cudaGetLastError();
@@ -687,6 +748,10 @@ cudaError_t launch_grad_norm(const OptTensor* t, int count, double* partial, int
     return norm_part<kOptTensors>(t, count, partial, first, last, ticket, norm, norm32, s);
 }
 
-long long opt_chunks(long long n) { return (n + kChunk - 1) / kChunk; }
+// (of the smallest kind)
+long long opt_chunks(long long n) {
+    constexpr int least = kStepThreads<8> * kLane;
+    return (n + least - 1) / least;
+}
 
 }  // namespace fcqt
