@@ -69,6 +69,30 @@ __host__ __device__ __forceinline__ unsigned mix32(unsigned x) {
     return x ^ (x >> 16);
 }
 
+// Two 32-bit floats in one instruction (sm_100), each rounded by itself.
+struct F2 {
+    unsigned long long w;
+};
+__device__ __forceinline__ F2 two(float a, float b) {
+    F2 x;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(x.w) : "f"(a), "f"(b));
+    return x;
+}
+__device__ __forceinline__ F2 two(float a) { return two(a, a); }
+__device__ __forceinline__ void split(F2 x, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.w));
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+    F2 x;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(x.w) : "l"(a.w), "l"(b.w));
+    return x;
+}
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+    F2 x;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(x.w) : "l"(a.w), "l"(b.w));
+    return x;
+}
+
 // the largest of three, NaN if one of them is
 __device__ __forceinline__ float max_nan(float a, float b, float c) {
     float y;
@@ -196,15 +220,15 @@ __device__ __forceinline__ void store_codes(uint8_t* p, int vec, int n, uint2 c)
             if (i < n) p[i] = (uint8_t)((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
     }
 }
-// sqrt(x + 2^-126) and a / b to 2^-22
+// square root and reciprocal to one unit in the last place
 __device__ __forceinline__ float root_of(float x) {
     float y;
-    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(__fadd_rn(x, 0x1p-126f)));
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float quotient(float a, float b) {
+__device__ __forceinline__ float one_over(float x) {
     float y;
-    asm("div.approx.ftz.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 // 8 values to codes, the first in the low byte
@@ -229,8 +253,7 @@ __device__ __forceinline__ void decode8(uint2 c, float s, float (&x)[8]) {
         const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(
             (__nv_fp8x2_storage_t)((i & 1) ? w >> 16 : w & 0xffffu), F);
         const float2 f = __half22float2(__half2(h));
-        x[2 * i] = __fmul_rn(f.x, s);
-        x[2 * i + 1] = __fmul_rn(f.y, s);
+        split(two(f.x, f.y) * two(s), x[2 * i], x[2 * i + 1]);
     }
 }
 // 2^(byte - 127); a byte of 0 is the subnormal 2^-127
@@ -282,29 +305,40 @@ __device__ __forceinline__ void encode_moments(const float (&m)[8], const float 
     const unsigned first = mix_first(index ^ key);
     float a[8], b[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const unsigned h = mix_middle(first ^ i);
-        // hm and hv: the low and the high half of mix32's result (its last step
-        // folds the high half into the low one) in the upper 16 bits, and half a
-        // step below.  The high half of a product with 2^20 (2^21) is that
-        // shifted to where the noise goes; it runs beside the integer adders
-        // and shifters, which are what this kernel has least of.
-        const unsigned hm = (((h << 16) ^ h) & 0xffff0000u) | 0x8000u;
-        const unsigned hv = (h & 0xffff0000u) | 0x8000u;
-        const unsigned mb = mad_hi(hm, k.two20, __float_as_uint(__fmul_rn(m[i], mi)));
-        const unsigned vb = mad_hi(hv, k.two21, __float_as_uint(__fmul_rn(v[i], vi)));
-        a[i] = __uint_as_float(mb & 0xfff00000u);
-        b[i] = __uint_as_float(vb & 0xffe00000u);
-        if constexpr (RARE) {
-            const float mmost = mk == 247 ? 240.f : 448.f, vmost = vk == 240 ? 28672.f : 57344.f;
-            a[i] = fminf(fmaxf(a[i], -mmost), mmost);
-            b[i] = fminf(b[i], vmost);
+    for (int i = 0; i < 8; i += 2) {
+        split(two(m[i], m[i + 1]) * two(mi), a[i], a[i + 1]);
+        split(two(v[i], v[i + 1]) * two(vi), b[i], b[i + 1]);
+#pragma unroll
+        for (int j = i; j < i + 2; ++j) {
+            const unsigned h = mix_middle(first ^ j);
+            // hm and hv: the low and the high half of mix32's result (its last
+            // step folds the high half into the low one) in the upper 16 bits,
+            // and half a step below.  The high half of a product with 2^20
+            // (2^21) is that shifted to where the noise goes; it runs beside
+            // the integer adders and shifters, which are what this kernel has
+            // least of.
+            const unsigned hm = (((h << 16) ^ h) & 0xffff0000u) | 0x8000u;
+            const unsigned hv = (h & 0xffff0000u) | 0x8000u;
+            a[j] = __uint_as_float(mad_hi(hm, k.two20, __float_as_uint(a[j])) & 0xfff00000u);
+            b[j] = __uint_as_float(mad_hi(hv, k.two21, __float_as_uint(b[j])) & 0xffe00000u);
+            if constexpr (RARE) {
+                const float mmost = mk == 247 ? 240.f : 448.f, vmost = vk == 240 ? 28672.f : 57344.f;
+                a[j] = fminf(fmaxf(a[j], -mmost), mmost);
+                b[j] = fminf(b[j], vmost);
+            }
         }
         // below the smallest normal value: 0 for m, that value for v.  |a| is at
         // most 1.875 * 2^-7 or at least 2^-6, its square 0.88 * 2^-12 or 2^-12:
         // a factor of 0 or 1, again beside the adders
-        a[i] = __fmul_rn(a[i], __saturatef(fmaf(__fmul_rn(a[i], a[i]), 0x1p40f, -0.94f * 0x1p28f)));
-        b[i] = fmaxf(b[i], fminf(__fmul_rn(__fmul_rn(v[i], 0x1p100f), 0x1p100f), 0x1p-14f));
+        const F2 ai = two(a[i], a[i + 1]);
+        float qa, qb, la, lb;
+        split(ai * ai, qa, qb);
+        qa = __saturatef(fmaf(qa, 0x1p40f, -0.94f * 0x1p28f));
+        qb = __saturatef(fmaf(qb, 0x1p40f, -0.94f * 0x1p28f));
+        split(ai * two(qa, qb), a[i], a[i + 1]);
+        split(two(v[i], v[i + 1]) * two(0x1p100f) * two(0x1p100f), la, lb);
+        b[i] = fmaxf(b[i], fminf(la, 0x1p-14f));
+        b[i + 1] = fmaxf(b[i + 1], fminf(lb, 0x1p-14f));
     }
     mc = to_fp8<__NV_E4M3>(a);
     vc = to_fp8<__NV_E5M2>(b);
@@ -363,22 +397,27 @@ __device__ __forceinline__ void update8(const OptTensor& t, const Chunk<T, BITS,
         unpack(c.m, m);
         unpack(c.v, v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            m[i] = __fmul_rn(m[i], a.b1);
-            v[i] = __fmul_rn(v[i], a.b2);
+        for (int i = 0; i < 8; i += 2) {
+            split(two(m[i], m[i + 1]) * two(a.b1), m[i], m[i + 1]);
+            split(two(v[i], v[i + 1]) * two(a.b2), v[i], v[i + 1]);
         }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float gi = __fmul_rn(g[i], s.clip);
-        m[i] = __fadd_rn(m[i], __fmul_rn(gi, a.omb1));
-        v[i] = __fadd_rn(v[i], __fmul_rn(__fmul_rn(gi, gi), a.omb2));
-        // root and quotient to 2^-22: their last bits are far below the
+    for (int i = 0; i < 8; i += 2) {
+        const F2 gi = two(g[i], g[i + 1]) * two(s.clip);
+        const F2 mi = two(m[i], m[i + 1]) + gi * two(a.omb1);
+        const F2 vi = two(v[i], v[i + 1]) + gi * gi * two(a.omb2);
+        // root and reciprocal to 2^-23: their last bits are far below the
         // parameter's own, and correctly rounded ones took a third of all
         // instructions.  2^-126 under the root keeps what is subnormal
         // from being read as 0 (above 2^-102 it changes nothing).
-        const float d = __fadd_rn(__fmul_rn(root_of(v[i]), s.root), a.eps);
-        p[i] = __fsub_rn(__fmul_rn(p[i], s.decay), __fmul_rn(quotient(m[i], d), s.rate));
+        float ra, rb, da, db;
+        split(vi + two(0x1p-126f), ra, rb);
+        split(two(root_of(ra), root_of(rb)) * two(s.root) + two(a.eps), da, db);
+        const F2 step = mi * two(one_over(da), one_over(db)) * two(-s.rate);
+        split(two(p[i], p[i + 1]) * two(s.decay) + step, p[i], p[i + 1]);
+        split(mi, m[i], m[i + 1]);
+        split(vi, v[i], v[i + 1]);
     }
     uint2 mc, vc;
     int mk, vk;

@@ -19,10 +19,10 @@ def step(p, g, m, v, t, lr, b1, b2, eps, wd, clip=1.0):
     4 U.  lr over it: lr 1, the quotient 1: 6 U.  One over its root: half of 4,
     and rsqrtf 4 (two units): 6 U.
     The denominator: half of v's 8, the root 2 (sqrt.approx.f32 is good to
-    2^-23), the constant 6 and its product 1, the sum 1: 14 U.  The quotient
-    adds 4 (div.approx.f32 is good to two units in the last place, 2^-22), the
-    rate 6 and its product 1: 25 U of the update beside m's own.  p: decay and
-    its product 2, the difference 1 on either side: 3 U |p| + (25 + 1 + 5) U
+    2^-23), the constant 6 and its product 1, the sum 1: 14 U.  One over it
+    adds 2 (rcp.approx.f32 is good to 2^-23), its product with m 1, the rate 6
+    and its product 1: 24 U of the update beside m's own.  p: decay and its
+    product 2, the difference 1 on either side: 3 U |p| + (24 + 1 + 5) U
     update(|m| terms).  Second orders are below a tenth of U: every count is
     raised by one.  (The root is that of v + 2^-126: below 1e-11 of eps.)"""
     g = g * clip
@@ -34,7 +34,7 @@ def step(p, g, m, v, t, lr, b1, b2, eps, wd, clip=1.0):
     p1 = p * (1 - lr * wd) - rate * m1 / d
     # the smallest values are rounded to multiples of 2^-149 instead
     tiny = 2.0 ** -148
-    return p1, m1, v1, (U * (4 * np.abs(p) + 32 * rate * mabs / d) + tiny, 6 * U * mabs + tiny,
+    return p1, m1, v1, (U * (4 * np.abs(p) + 31 * rate * mabs / d) + tiny, 6 * U * mabs + tiny,
                         9 * U * v1 + tiny)
 
 
