@@ -280,7 +280,6 @@ struct OptArgs {
     float b1, omb1, b2, omb2, eps;
     float ln1, ln2;            // logarithms of the betas
     unsigned seed_key;
-    unsigned two20, two21;     // 2^20 and 2^21, not known when the kernel is compiled
 };
 
 // one launch over 1 to kOptTensors tensors of one type, all with a master copy

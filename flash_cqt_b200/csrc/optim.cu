@@ -37,12 +37,11 @@ namespace {
 
 constexpr int kLane = 8;                        // consecutive elements a thread
 static_assert(32 * kLane == kOptBlock, "a warp is one block");
-// CTA sizes.  The step: 28 warps an SM with 72 registers for 8-bit moments, 16
-// with 128 for 32-bit ones, which move more bytes an element.  Measured, 67 M
-// float elements with 8-bit moments: 174 us with 4 CTAs of 224 threads an SM
-// (172 with 2 of 448), 211 with 3 of 256, 225 with 4 of 192, 239 with 5 of 192;
-// 32-bit moments of 144 M bf16 elements: 660 us with 16 warps an SM, 675 with
-// 24, 750 with 32: what more loads in flight win they lose in DRAM pages.
+// CTA sizes.  Measured: 67 M float elements with 8-bit moments, 188 us with 4
+// CTAs of 224 threads an SM (72 registers), 188 with 3 of 256, 217 with 4 of 256
+// (64, some spilled); 96 M bf16 ones 219, 225 and 215 us.  32-bit moments move
+// more bytes an element and want fewer threads: 144 M bf16 elements with a master
+// copy 660 us with 16 warps an SM, 675 with 24, 750 with 32.
 template <int BITS>
 constexpr int kStepThreads = BITS == 8 ? 224 : 256;
 template <int BITS>
@@ -97,11 +96,6 @@ __device__ __forceinline__ F2 operator+(F2 a, F2 b) {
 __device__ __forceinline__ float max_nan(float a, float b, float c) {
     float y;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-    return y;
-}
-__device__ __forceinline__ unsigned mad_hi(unsigned a, unsigned b, unsigned c) {
-    unsigned y;
-    asm("mad.hi.u32 %0, %1, %2, %3;" : "=r"(y) : "r"(a), "r"(b), "r"(c));
     return y;
 }
 
@@ -280,8 +274,8 @@ struct StepScalars {
 template <bool RARE>
 __device__ __forceinline__ void encode_moments(const float (&m)[8], const float (&v)[8], int n,
                                                unsigned mtop, unsigned vtop, unsigned index,
-                                               unsigned key, const OptArgs& k, uint2& mc,
-                                               uint2& vc, int& mk, int& vk) {
+                                               unsigned key, uint2& mc, uint2& vc, int& mk,
+                                               int& vk) {
     if constexpr (RARE) {
         mtop = vtop = 0;
 #pragma unroll
@@ -311,16 +305,12 @@ __device__ __forceinline__ void encode_moments(const float (&m)[8], const float 
 #pragma unroll
         for (int j = i; j < i + 2; ++j) {
             const unsigned h = mix_middle(first ^ j);
-            // hm and hv: the low and the high half of mix32's result (its last
-            // step folds the high half into the low one) in the upper 16 bits,
-            // and half a step below.  The high half of a product with 2^20
-            // (2^21) is that shifted to where the noise goes; it runs beside
-            // the integer adders and shifters, which are what this kernel has
-            // least of.
-            const unsigned hm = (((h << 16) ^ h) & 0xffff0000u) | 0x8000u;
-            const unsigned hv = (h & 0xffff0000u) | 0x8000u;
-            a[j] = __uint_as_float(mad_hi(hm, k.two20, __float_as_uint(a[j])) & 0xfff00000u);
-            b[j] = __uint_as_float(mad_hi(hv, k.two21, __float_as_uint(b[j])) & 0xffe00000u);
+            // the low and the high half of mix32's result (its last step folds
+            // the high half into the low one), and half a step below
+            const unsigned hm = (((h << 4) ^ (h >> 12)) & 0xffff0u) + 8u;
+            const unsigned hv = ((h >> 11) & 0x1fffe0u) + 16u;
+            a[j] = __uint_as_float((__float_as_uint(a[j]) + hm) & 0xfff00000u);
+            b[j] = __uint_as_float((__float_as_uint(b[j]) + hv) & 0xffe00000u);
             if constexpr (RARE) {
                 const float mmost = mk == 247 ? 240.f : 448.f, vmost = vk == 240 ? 28672.f : 57344.f;
                 a[j] = fminf(fmaxf(a[j], -mmost), mmost);
@@ -329,7 +319,8 @@ __device__ __forceinline__ void encode_moments(const float (&m)[8], const float 
         }
         // below the smallest normal value: 0 for m, that value for v.  |a| is at
         // most 1.875 * 2^-7 or at least 2^-6, its square 0.88 * 2^-12 or 2^-12:
-        // a factor of 0 or 1, again beside the adders
+        // a factor of 0 or 1, worked out beside the integer adders, which this
+        // kernel has least of
         const F2 ai = two(a[i], a[i + 1]);
         float qa, qb, la, lb;
         split(ai * ai, qa, qb);
@@ -362,7 +353,6 @@ struct Chunk {
     Raw8<P> p;
     Raw8<float> m, v;   // BITS 32
     uint2 mc, vc;       // BITS 8
-    uint8_t ms, vs;
 
     __device__ __forceinline__ void load(const OptTensor& t, long long at, int n, int vec) {
         base = at;
@@ -372,9 +362,6 @@ struct Chunk {
         if constexpr (BITS == 8) {
             mc = load_codes(static_cast<const uint8_t*>(t.m) + base, vec, n);
             vc = load_codes(static_cast<const uint8_t*>(t.v) + base, vec, n);
-            // a lane behind the tensor's end may be behind the scales' end too
-            ms = n > 0 ? t.ms[base / kOptBlock] : 1;
-            vs = n > 0 ? t.vs[base / kOptBlock] : 1;
         } else {
             load8(static_cast<const float*>(t.m) + base, vec, n, m);
             load8(static_cast<const float*>(t.v) + base, vec, n, v);
@@ -385,14 +372,14 @@ struct Chunk {
 template <class T, int BITS, bool MASTER>
 __device__ __forceinline__ void update8(const OptTensor& t, const Chunk<T, BITS, MASTER>& c,
                                         const OptArgs& a, const StepScalars& s, unsigned key,
-                                        int n, int vec) {
+                                        int n, int vec, uint8_t* ms, uint8_t* vs) {
     float g[8], p[8], m[8], v[8];
     unpack(c.g, g);
     unpack(c.p, p);
     if constexpr (BITS == 8) {
         // the scales are powers of two: b (code s) = code (b s)
-        decode8<__NV_E4M3>(c.mc, __fmul_rn(scale_of(c.ms), a.b1), m);
-        decode8<__NV_E5M2>(c.vc, __fmul_rn(scale_of(c.vs), a.b2), v);
+        decode8<__NV_E4M3>(c.mc, __fmul_rn(scale_of(*ms), a.b1), m);
+        decode8<__NV_E5M2>(c.vc, __fmul_rn(scale_of(*vs), a.b2), v);
     } else {
         unpack(c.m, m);
         unpack(c.v, v);
@@ -433,20 +420,18 @@ __device__ __forceinline__ void update8(const OptTensor& t, const Chunk<T, BITS,
         const unsigned vtop = __reduce_max_sync(0xffffffffu, __float_as_uint(vmax));
         // above 1.75 * 2^127 the scales are the largest (or there is none)
         if (max(mtop, vtop) > 0x7f600000u)
-            encode_moments<true>(m, v, n, mtop, vtop, (unsigned)c.base, key, a, mc, vc, mk, vk);
+            encode_moments<true>(m, v, n, mtop, vtop, (unsigned)c.base, key, mc, vc, mk, vk);
         else
-            encode_moments<false>(m, v, n, mtop, vtop, (unsigned)c.base, key, a, mc, vc, mk, vk);
+            encode_moments<false>(m, v, n, mtop, vtop, (unsigned)c.base, key, mc, vc, mk, vk);
     }
-    // all stores together: the parameter's ahead of the moments' rounding made
-    // 67 M elements take 229 us instead of 174
     if constexpr (MASTER) store8(t.master + c.base, vec, n, p);
     store8(static_cast<T*>(t.p) + c.base, vec, n, p);
     if constexpr (BITS == 8) {
         store_codes(static_cast<uint8_t*>(t.m) + c.base, vec, n, mc);
         store_codes(static_cast<uint8_t*>(t.v) + c.base, vec, n, vc);
-        if ((threadIdx.x & 31) == 0 && n > 0) {
-            t.ms[c.base / kOptBlock] = (uint8_t)mk;
-            t.vs[c.base / kOptBlock] = (uint8_t)vk;
+        if ((threadIdx.x & 31) == 0) {
+            *ms = (uint8_t)mk;
+            *vs = (uint8_t)vk;
         }
     } else {
         store8(static_cast<float*>(t.m) + c.base, vec, n, m);
@@ -457,13 +442,14 @@ __device__ __forceinline__ void update8(const OptTensor& t, const Chunk<T, BITS,
 // a chunk that the tensor ends in, or whose arrays are not aligned
 template <class T, int BITS, bool MASTER>
 __device__ __forceinline__ void update_part(const OptTensor& t, long long base, const OptArgs& a,
-                                         const StepScalars& s, unsigned key) {
+                                            const StepScalars& s, unsigned key, uint8_t* ms,
+                                            uint8_t* vs) {
     const long long left = t.n - base;
     const int n = left >= 8 ? 8 : (left > 0 ? (int)left : 0);
     const int vec = n == 8 ? t.vec : 0;
     Chunk<T, BITS, MASTER> c;
     c.load(t, base, n, vec);
-    update8(t, c, a, s, key, n, vec);
+    update8(t, c, a, s, key, n, vec, ms, vs);
 }
 
 // the tensor that chunk c lies in: the last one whose first chunk is <= c
@@ -498,6 +484,7 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
     constexpr int kThreads = kStepThreads<BITS>, kChunk = kThreads * kLane;
     __shared__ TensorPlan tensor[N];
     __shared__ int chunk[kThreads];      // tensor of each of the CTA's next chunks, and kWhole
+    __shared__ uint8_t scale[2][BITS == 8 ? kThreads * (kThreads / 32) : 1];
     __shared__ long long steps[N];
     __shared__ StepScalars same;
     __shared__ unsigned order;
@@ -528,8 +515,11 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
         steps[i] = step;
     }
     // tensors are looked up by one thread a chunk, a CTA's width at a time (the
-    // last of a width is the first of the next)
+    // last one of a width is the first of the next).  The scale bytes of a width
+    // are read and written together: a byte at a time from every warp, 32 of
+    // them to a sector of the L2 cache, cost a quarter of the kernel's time.
     constexpr unsigned kWidth = kThreads - 1;
+    constexpr int kWarps = kThreads / 32;
     for (unsigned c0 = blockIdx.x; c0 < tab.chunks; c0 += kWidth * gridDim.x) {
         __syncthreads();
         const unsigned long long mine = c0 + (unsigned long long)threadIdx.x * gridDim.x;
@@ -543,9 +533,27 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
             chunk[threadIdx.x] = lo | (is_whole<kChunk>(tab.t[lo], (unsigned)mine) ? kWhole : 0);
         }
         __syncthreads();
+        const unsigned left = (tab.chunks - c0 - 1) / gridDim.x + 1;
+        const unsigned width = left < kWidth ? left : kWidth;
+        // calls f(place in shared memory, tensor, block) for every block
+        const auto each_block = [&](auto f) {
+            for (unsigned i = threadIdx.x; i < width * kWarps; i += kThreads) {
+                const unsigned k = i / kWarps, w = i - k * kWarps;
+                const OptTensor& t = tab.t[chunk[k] & ~kWhole];
+                const long long block = (long long)(c0 + k * gridDim.x - t.chunk0) * kWarps + w;
+                if (block * kOptBlock < t.n) f(i, t, block);
+            }
+        };
+        if constexpr (BITS == 8) {
+            each_block([&](unsigned i, const OptTensor& t, long long block) {
+                scale[0][i] = t.ms[block];
+                scale[1][i] = t.vs[block];
+            });
+            __syncthreads();
+        }
         StepScalars s = same;
         unsigned c = c0;
-        for (unsigned k = 0; k < kWidth && c < tab.chunks; ++k, c += gridDim.x) {
+        for (unsigned k = 0; k < width; ++k, c += gridDim.x) {
             const int i = chunk[k];
             const OptTensor& t = tab.t[i & ~kWhole];
             const TensorPlan q = tensor[i & ~kWhole];
@@ -560,9 +568,18 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
             }
             const long long base = (long long)(c - q.chunk0) * kChunk + lane;
             const unsigned key = BITS == 8 ? mix32(q.key + (unsigned)(base >> 32)) : 0;
-            if (i & kWhole) update8(t, here, a, s, key, 8, 2);
-            else update_part<T, BITS, MASTER>(t, base, a, s, key);
+            uint8_t* ms = &scale[0][BITS == 8 ? k * kWarps + threadIdx.x / 32 : 0];
+            uint8_t* vs = &scale[1][BITS == 8 ? k * kWarps + threadIdx.x / 32 : 0];
+            if (i & kWhole) update8(t, here, a, s, key, 8, 2, ms, vs);
+            else update_part<T, BITS, MASTER>(t, base, a, s, key, ms, vs);
             here = next;
+        }
+        if constexpr (BITS == 8) {
+            __syncthreads();
+            each_block([&](unsigned i, const OptTensor& t, long long block) {
+                t.ms[block] = scale[0][i];
+                t.vs[block] = scale[1][i];
+            });
         }
     }
     // every CTA has read the counts: the last one to come here advances them
@@ -771,8 +788,6 @@ constexpr int kSmall = 12, kMiddle = 100;
 
 cudaError_t launch_adamw(const OptTensor* t, int count, int bits, OptArgs a, cudaStream_t s) {
     a.seed_key = mix32(a.seed_key);
-    a.two20 = 1u << 20;
-    a.two21 = 1u << 21;
     if (count <= kSmall) return adamw_typed<kSmall>(t, count, bits, a, s);
     if (count <= kMiddle) return adamw_typed<kMiddle>(t, count, bits, a, s);
     return adamw_typed<kOptTensors>(t, count, bits, a, s);
