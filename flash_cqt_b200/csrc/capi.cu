@@ -939,8 +939,8 @@ int cqt_sliced_adj_analysis(const cqt_tables* t, const float* gcoef, const cqt_s
 }
 
 // ---- AdamW over many tensors (optim.cu)
-// workspace: [0] the ticket, [8] the norm in 64 bits, [256] one partial sum per
-// CTA of each launch
+// workspace: [0] the norm's ticket, [4] the step's, [8] the norm in 64 bits, [16]
+// in 32, [256] one partial sum per CTA of each launch of the norm
 static size_t adamw_ws(int count) {
     const size_t launches = ((size_t)count + kOptTensors - 1) / kOptTensors;
     return kWsHeader + launches * kNormCtas * sizeof(double);
@@ -1040,6 +1040,7 @@ int cqt_adamw_step(const cqt_adamw_tensor* tensors, int count, int state_bits,
     if (!(a->beta1 >= 0 && a->beta1 < 1 && a->beta2 >= 0 && a->beta2 < 1) || !(a->eps >= 0))
         return fail(CQT_ERR_ARG, "betas must lie in [0, 1) and eps must not be negative");
     if (!a->lr_dev && !(a->lr >= 0)) return fail(CQT_ERR_ARG, "lr must not be negative");
+    if (a->use_norm < 0 || a->use_norm > 2) return fail(CQT_ERR_ARG, "use_norm must be 0, 1 or 2");
     if (a->use_norm && !(a->max_norm > 0)) return fail(CQT_ERR_ARG, "max_norm must be positive");
     OptArgs o{};
     o.lr = a->lr;
@@ -1050,7 +1051,8 @@ int cqt_adamw_step(const cqt_adamw_tensor* tensors, int count, int state_bits,
     o.norm = a->use_norm
                  ? reinterpret_cast<const double*>(static_cast<char*>(workspace) + 8) : nullptr;
     o.max_norm = a->max_norm;
-    o.ticket = static_cast<unsigned*>(workspace);
+    o.behind_norm = a->use_norm == 2;
+    o.ticket = static_cast<unsigned*>(workspace) + 1;
     o.b1 = (float)a->beta1;
     o.omb1 = (float)(1.0 - a->beta1);
     o.b2 = (float)a->beta2;
@@ -1072,6 +1074,7 @@ int cqt_adamw_step(const cqt_adamw_tensor* tensors, int count, int state_bits,
             if (n == 0) break;
             const cudaError_t e =
                 launch_adamw(part, n, state_bits, o, static_cast<cudaStream_t>(stream));
+            o.behind_norm = 0;
             if (e != cudaSuccess) return cuda_fail(e, "adamw launch");
         }
     }

@@ -276,6 +276,7 @@ struct OptArgs {
     const float* lr_dev;       // not null: the rate is read from the device
     const double* norm;        // not null: gradients are scaled to max_norm
     double max_norm;
+    int behind_norm;           // the launch before this one was the norm's last
     unsigned* ticket;          // zero between launches
     float b1, omb1, b2, omb2, eps;
     float ln1, ln2;            // logarithms of the betas

@@ -497,6 +497,7 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
     if (is_whole<kChunk>(tab.t[first], blockIdx.x))
         here.load(tab.t[first], (long long)(blockIdx.x - tab.t[first].chunk0) * kChunk + lane, 8, 2);
     if (threadIdx.x == kThreads - 1) {
+        if (a.norm) pdl_wait();   // what else this kernel reads, the norm's does not write
         same.decay = (float)(1.0 - (a.lr_dev ? (double)*a.lr_dev : a.lr) * a.wd);
         const double c = a.norm ? a.max_norm / (*a.norm + 1e-6) : 1.0;
         same.clip = c > 1.0 ? 1.f : (float)c;   // NaN stays NaN
@@ -628,14 +629,22 @@ __global__ void __launch_bounds__(kNormThreads)
 norm_kernel(const __grid_constant__ OptTable<N> tab, double* partial, int first, int last,
             unsigned* ticket, double* norm, float* norm32) {
     constexpr int kChunk = kNormThreads * kLane;
+    __shared__ unsigned chunk0[N];
     __shared__ int tensor[kNormThreads];   // of each of the CTA's next chunks, and kWhole
+    pdl_launch_dependents();
+    for (int i = threadIdx.x; i < tab.count; i += kNormThreads) chunk0[i] = tab.t[i].chunk0;
     double part[4] = {0, 0, 0, 0};
     for (unsigned c0 = blockIdx.x; c0 < tab.chunks; c0 += kNormThreads * gridDim.x) {
         __syncthreads();
         const unsigned long long mine = c0 + (unsigned long long)threadIdx.x * gridDim.x;
         if (mine < tab.chunks) {
-            const int i = find_tensor(tab, (unsigned)mine);
-            tensor[threadIdx.x] = i | (is_whole<kChunk>(tab.t[i], (unsigned)mine) ? kWhole : 0);
+            int lo = 0, hi = tab.count - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (chunk0[mid] <= (unsigned)mine) lo = mid;
+                else hi = mid - 1;
+            }
+            tensor[threadIdx.x] = lo | (is_whole<kChunk>(tab.t[lo], (unsigned)mine) ? kWhole : 0);
         }
         __syncthreads();
         // four chunks on their way at a time, where all of them are whole
@@ -748,8 +757,9 @@ cudaError_t adamw_launch(const OptTensor* t, int count, const OptArgs& a, cudaSt
     OptTable<N> tab;
     fill(&tab, t, count, kThreads * kLane);
     static const unsigned most = resident_ctas(adamw_kernel<N, T, BITS, MASTER>, kThreads);
-    adamw_kernel<N, T, BITS, MASTER><<<opt_grid(tab.chunks, most), kThreads, 0, s>>>(tab, a);
-    return cudaGetLastError();
+    // right behind the norm, the kernel may start on what the norm leaves free
+    return launch_pdl(a.behind_norm, adamw_kernel<N, T, BITS, MASTER>, dim3(opt_grid(tab.chunks, most)),
+                      dim3(kThreads), 0, s, tab, a);
 }
 
 template <int N, class T, bool MASTER>

@@ -664,7 +664,7 @@ struct AdamWPlan {
             TORCH_CHECK(rc == 0, what, " failed (", rc, "): ", last_error());
         };
         cqt_adamw_args a{};
-        a.use_norm = max_norm.is_none() ? 0 : 1;
+        a.use_norm = max_norm.is_none() ? 0 : 2;   // 1 after the first launch behind the norm
         a.max_norm = a.use_norm ? number(max_norm.ptr()) : 0.0;
         a.seed = seed;
         if (a.use_norm)
@@ -705,6 +705,7 @@ struct AdamWPlan {
             check(step_fn(todo.data() + first, (int)(last - first), bits, &a, ws.data_ptr(),
                           (size_t)ws.numel(), stream),
                   "cqt_adamw_step");
+            if (a.use_norm) a.use_norm = 1;
             first = last;
         }
         keep.clear();

@@ -365,6 +365,7 @@ class AdamW(torch.optim.Optimizer):
                 (_native.CqtAdamwTensor * sum(map(len, lists)))(*(t for x in lists for t in x)))
             _native._check(L.cqt_grad_norm(every, len(every), self.grad_norm.data_ptr(),
                                            ws.data_ptr(), ws.numel(), stream), "cqt_grad_norm")
+        use_norm = 0 if self.max_norm is None else 2   # 1 after the launch behind the norm
         for g, todo in zip(self.param_groups, lists):
             if not len(todo):
                 continue
@@ -373,9 +374,10 @@ class AdamW(torch.optim.Optimizer):
             args = _native.CqtAdamwArgs(
                 0.0 if on_device else float(lr), *map(float, g["betas"]), float(g["eps"]),
                 float(g["weight_decay"]), self.max_norm or 0.0,
-                lr.data_ptr() if on_device else None, int(self.max_norm is not None), self.seed)
+                lr.data_ptr() if on_device else None, use_norm, self.seed)
             _native._check(L.cqt_adamw_step(todo, len(todo), g["state_bits"], ctypes.byref(args),
                                             ws.data_ptr(), ws.numel(), stream), "cqt_adamw_step")
+            use_norm = min(use_norm, 1)
 
 
 _hooked_step = torch.optim.Optimizer.profile_hook_step(AdamW._step)

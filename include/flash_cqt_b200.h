@@ -342,8 +342,10 @@ typedef struct cqt_adamw_args {
     double lr, beta1, beta2, eps, weight_decay;
     double max_norm;            /* with use_norm */
     const float* lr_dev;        /* not NULL: the rate is read from the device */
-    int32_t use_norm;           /* scale by the norm that cqt_grad_norm left in
-                                   the workspace */
+    int32_t use_norm;           /* 1: scale by the norm that cqt_grad_norm left in
+                                   the workspace; 2: the same, and cqt_grad_norm
+                                   was the last call on the stream (the step then
+                                   starts before the norm has ended) */
     uint32_t seed;
 } cqt_adamw_args;
 

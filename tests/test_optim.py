@@ -85,6 +85,10 @@ def test_c_entries_refuse():
         assert "betas" in step(T(**ok), a)[1]
     a = _native.CqtAdamwArgs(1e-3, 0.9, 0.999, 1e-8, 0.0, 0.0, None, 1, 0)
     assert step(T(**ok), a)[1] == "max_norm must be positive"
+    a = _native.CqtAdamwArgs(1e-3, 0.9, 0.999, 1e-8, 0.0, 1.0, None, 3, 0)
+    assert "use_norm" in step(T(**ok), a)[1]
+    a = _native.CqtAdamwArgs(-1e-3, 0.9, 0.999, 1e-8, 0.0, 1.0, None, 0, 0)
+    assert step(T(**ok), a)[1] == "lr must not be negative"
     assert L.cqt_grad_norm(ctypes.byref(T(numel=3)), 1, None, at, need, None) == -1
     assert L.cqt_grad_norm(None, 1, None, at, need, None) == -1
     # a list without elements is no work
