@@ -252,7 +252,7 @@ __device__ __forceinline__ void store_v8(float* p, const float (&x)[8]) {
 // AdamW over many tensors (optim.cu)
 constexpr int kOptBlock = 256;     // elements that share a scale (8-bit moments)
 constexpr int kOptTensors = 360;   // tensors in one launch (32 KB of kernel parameters)
-constexpr int kNormCtas = 148 * 4; // CTAs of one launch of the norm at most
+constexpr int kNormCtas = 148 * 8; // CTAs of one launch of the norm at most
 enum OptType { kOptF32 = 0, kOptBf16 = 1, kOptF16 = 2 };
 
 struct OptTensor {

@@ -466,10 +466,23 @@ __device__ __forceinline__ int find_tensor(const OptTable<N>& tab, unsigned c) {
 
 constexpr int kWhole = 1 << 30;   // every thread has 8 aligned elements
 
-// whether chunk c of the tensor has all its elements, aligned
+// the chunks of a tensor before this one have all their elements, aligned
 template <int CHUNK>
-__device__ __forceinline__ bool is_whole(const OptTensor& t, unsigned c) {
-    return t.vec == 2 && (long long)(c - t.chunk0 + 1) * CHUNK <= t.n;
+__device__ __forceinline__ unsigned whole_end(const OptTensor& t) {
+    return t.chunk0 + (t.vec == 2 ? (unsigned)(t.n / CHUNK) : 0);
+}
+
+// what the chunks need of their tensors is copied to shared memory first:
+// threads that look at different tensors would take turns at the parameters
+template <class Of>   // the first chunk of tensor i
+__device__ __forceinline__ int find_in(const Of& first, int count, unsigned c) {
+    int lo = 0, hi = count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (first(mid) <= c) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
 }
 
 struct TensorPlan {
@@ -485,6 +498,7 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
     __shared__ TensorPlan tensor[N];
     __shared__ int chunk[kThreads];      // tensor of each of the CTA's next chunks, and kWhole
     __shared__ uint8_t scale[2][BITS == 8 ? kThreads * (kThreads / 32) : 1];
+    __shared__ unsigned whole[N];
     __shared__ long long steps[N];
     __shared__ StepScalars same;
     __shared__ unsigned order;
@@ -494,7 +508,7 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
     Chunk<T, BITS, MASTER> here;
     const long long lane = threadIdx.x * kLane;
     const int first = find_tensor(tab, blockIdx.x);
-    if (is_whole<kChunk>(tab.t[first], blockIdx.x))
+    if (blockIdx.x < whole_end<kChunk>(tab.t[first]))
         here.load(tab.t[first], (long long)(blockIdx.x - tab.t[first].chunk0) * kChunk + lane, 8, 2);
     if (threadIdx.x == kThreads - 1) {
         if (a.norm) pdl_wait();   // what else this kernel reads, the norm's does not write
@@ -513,6 +527,7 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
         q.key = BITS == 8 ? mix32(mix32(a.seed_key + (unsigned)step) + (unsigned)t.ordinal) : 0;
         q.chunk0 = t.chunk0;
         tensor[i] = q;
+        whole[i] = whole_end<kChunk>(t);
         steps[i] = step;
     }
     // tensors are looked up by one thread a chunk, a CTA's width at a time (the
@@ -525,13 +540,8 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
         __syncthreads();
         const unsigned long long mine = c0 + (unsigned long long)threadIdx.x * gridDim.x;
         if (mine < tab.chunks) {
-            int lo = 0, hi = tab.count - 1;
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (tensor[mid].chunk0 <= (unsigned)mine) lo = mid;
-                else hi = mid - 1;
-            }
-            chunk[threadIdx.x] = lo | (is_whole<kChunk>(tab.t[lo], (unsigned)mine) ? kWhole : 0);
+            const int i = find_in([&](int m) { return tensor[m].chunk0; }, tab.count, (unsigned)mine);
+            chunk[threadIdx.x] = i | ((unsigned)mine < whole[i] ? kWhole : 0);
         }
         __syncthreads();
         const unsigned left = (tab.chunks - c0 - 1) / gridDim.x + 1;
@@ -594,22 +604,23 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
 
 // ---- sqrt(sum of squares over all gradients), summed in 64 bits in a fixed
 // order: threads, warps, CTAs, launches
+// a thread's 8 elements of a chunk, some of them or none
 template <class T>
-__device__ __forceinline__ void add_squares(const Raw8<T>& r, double (&sum)[4]) {
+__device__ __forceinline__ void squares8(const OptTensor& t, long long base, bool whole,
+                                         double (&sum)[4]) {
+    const T* g = static_cast<const T*>(t.g) + base;
+    Raw8<T> r;
+    if (whole) {
+        load8(g, 2, 8, r);
+    } else {
+        const long long left = t.n - base;
+        const int n = left >= 8 ? 8 : (left > 0 ? (int)left : 0);
+        load8(g, n == 8 ? t.vec : 0, n, r);
+    }
     float x[8];
     unpack(r, x);
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum[i & 3] = fma((double)x[i], (double)x[i], sum[i & 3]);
-}
-
-// the chunk's 8 elements of a thread, some of them or none
-template <class T>
-__device__ __forceinline__ void squares8(const OptTensor& t, long long base, double (&sum)[4]) {
-    const long long left = t.n - base;
-    const int n = left >= 8 ? 8 : (left > 0 ? (int)left : 0);
-    Raw8<T> r;
-    load8(static_cast<const T*>(t.g) + base, n == 8 ? t.vec : 0, n, r);
-    add_squares(r, sum);
 }
 
 __device__ __forceinline__ double cta_sum(double x) {
@@ -625,76 +636,34 @@ __device__ __forceinline__ double cta_sum(double x) {
 }
 
 template <int N>
-__global__ void __launch_bounds__(kNormThreads)
+__global__ void __launch_bounds__(kNormThreads, kNormCtas / 148)
 norm_kernel(const __grid_constant__ OptTable<N> tab, double* partial, int first, int last,
             unsigned* ticket, double* norm, float* norm32) {
     constexpr int kChunk = kNormThreads * kLane;
-    __shared__ unsigned chunk0[N];
+    __shared__ unsigned chunk0[N], whole[N];
     __shared__ int tensor[kNormThreads];   // of each of the CTA's next chunks, and kWhole
     pdl_launch_dependents();
-    for (int i = threadIdx.x; i < tab.count; i += kNormThreads) chunk0[i] = tab.t[i].chunk0;
+    for (int i = threadIdx.x; i < tab.count; i += kNormThreads) {
+        chunk0[i] = tab.t[i].chunk0;
+        whole[i] = whole_end<kChunk>(tab.t[i]);
+    }
     double part[4] = {0, 0, 0, 0};
     for (unsigned c0 = blockIdx.x; c0 < tab.chunks; c0 += kNormThreads * gridDim.x) {
         __syncthreads();
         const unsigned long long mine = c0 + (unsigned long long)threadIdx.x * gridDim.x;
         if (mine < tab.chunks) {
-            int lo = 0, hi = tab.count - 1;
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (chunk0[mid] <= (unsigned)mine) lo = mid;
-                else hi = mid - 1;
-            }
-            tensor[threadIdx.x] = lo | (is_whole<kChunk>(tab.t[lo], (unsigned)mine) ? kWhole : 0);
+            const int i = find_in([&](int m) { return chunk0[m]; }, tab.count, (unsigned)mine);
+            tensor[threadIdx.x] = i | ((unsigned)mine < whole[i] ? kWhole : 0);
         }
         __syncthreads();
-        // four chunks on their way at a time, where all of them are whole
-        constexpr unsigned kBatch = 4;
         unsigned c = c0;
-        for (unsigned k = 0; k < kNormThreads && c < tab.chunks;) {
-            const bool all = k + kBatch <= kNormThreads &&
-                             c + (unsigned long long)(kBatch - 1) * gridDim.x < tab.chunks &&
-                             (tensor[k] & tensor[k + 1] & tensor[k + 2] & tensor[k + 3] & kWhole);
-            if (all) {
-                float4 r[kBatch][2];
-#pragma unroll
-                for (unsigned j = 0; j < kBatch; ++j) {
-                    const OptTensor& t = tab.t[tensor[k + j] & ~kWhole];
-                    const long long base =
-                        (long long)(c + j * gridDim.x - t.chunk0) * kChunk + threadIdx.x * kLane;
-                    if (t.dtype == kOptF32) {
-                        float x[8];
-                        load_v8(static_cast<const float*>(t.g) + base, x);
-                        r[j][0] = make_float4(x[0], x[1], x[2], x[3]);
-                        r[j][1] = make_float4(x[4], x[5], x[6], x[7]);
-                    } else {
-                        r[j][0] = *reinterpret_cast<const float4*>(
-                            static_cast<const unsigned short*>(t.g) + base);
-                    }
-                }
-#pragma unroll
-                for (unsigned j = 0; j < kBatch; ++j) {
-                    const int d = tab.t[tensor[k + j] & ~kWhole].dtype;
-                    if (d == kOptF32) {
-                        add_squares(Raw8<float>{{r[j][0].x, r[j][0].y, r[j][0].z, r[j][0].w,
-                                                 r[j][1].x, r[j][1].y, r[j][1].z, r[j][1].w}}, part);
-                    } else {
-                        const uint4 w = make_uint4(__float_as_uint(r[j][0].x), __float_as_uint(r[j][0].y),
-                                                   __float_as_uint(r[j][0].z), __float_as_uint(r[j][0].w));
-                        if (d == kOptBf16) add_squares(Raw8<__nv_bfloat16>{w}, part);
-                        else add_squares(Raw8<__half>{w}, part);
-                    }
-                }
-                k += kBatch;
-                c += kBatch * gridDim.x;
-            } else {
-                const OptTensor& t = tab.t[tensor[k] & ~kWhole];
-                const long long base = (long long)(c - t.chunk0) * kChunk + threadIdx.x * kLane;
-                if (t.dtype == kOptF32) squares8<float>(t, base, part);
-                else if (t.dtype == kOptBf16) squares8<__nv_bfloat16>(t, base, part);
-                else squares8<__half>(t, base, part);
-                ++k;
-                c += gridDim.x;
-            }
+        for (int k = 0; k < kNormThreads && c < tab.chunks; ++k, c += gridDim.x) {
+            const int i = tensor[k];
+            const OptTensor& t = tab.t[i & ~kWhole];
+            const long long base = (long long)(c - t.chunk0) * kChunk + threadIdx.x * kLane;
+            if (t.dtype == kOptF32) squares8<float>(t, base, i & kWhole, part);
+            else if (t.dtype == kOptBf16) squares8<__nv_bfloat16>(t, base, i & kWhole, part);
+            else squares8<__half>(t, base, i & kWhole, part);
         }
     }
     double sum = (part[0] + part[1]) + (part[2] + part[3]);
