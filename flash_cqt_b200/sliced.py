@@ -24,6 +24,7 @@ import math
 
 import torch
 
+from .coefcache import CoefCache
 from .engine import SlicedEngine
 from .layout import periodic_hann
 from .oct_cqt import OctCQT
@@ -229,10 +230,11 @@ class SlicedCQT:
         out = out[..., 2 * H:]
         return out if length is None else out[..., :length]
 
-    def streamer(self, lead, device=None):
+    def streamer(self, lead, device=None, history=0, history_format="int8"):
         """a SliceStream (one CUDA graph replay per chunk) for chunks of
-        shape [*lead, hop]"""
-        return SliceStream(self, lead, device)
+        shape [*lead, hop]; history > 0 keeps the coefficients of the last
+        that many slices in 8 bits (``CoefCache``)"""
+        return SliceStream(self, lead, device, history, history_format)
 
     # streaming API, state of one half slice (sliced.py:171-209)
     #
@@ -330,9 +332,18 @@ class SliceStream:
     slice 1) and even k >= 2 (as slice 2); the rolls follow the parity.
     Results are bit-identical to ``stream_fwd`` / ``stream_bwd`` and to the
     whole-buffer transform.  Inference only (graphs record no autograd);
-    returned tensors are fresh copies."""
+    returned tensors are fresh copies.
 
-    def __init__(self, sliced, lead, device=None):
+    With ``history=n`` the forward graphs also write every slice's coefficients
+    into a ``CoefCache`` of n slices (``self.cache``), quantised to
+    ``history_format`` ("int8" or "e4m3") on the way, and ``past(k)`` reads the
+    last k of them back -- what a streaming model sees each hop:
+
+        st = sliced.streamer((B, C), history=64)
+        st.fwd(chunk)
+        blocks, side = st.past(32, dtype=torch.bfloat16)"""
+
+    def __init__(self, sliced, lead, device=None, history=0, history_format="int8"):
         dev = torch.device(device) if device is not None else sliced.device
         se = sliced._fused(dev)
         if se is None:
@@ -354,12 +365,18 @@ class SliceStream:
         self.ws = torch.zeros(max(se.eng.tables.workspace_bytes(rows), 256), dtype=torch.uint8,
                               device=dev)   # zeroed: the header holds the wait status
         self.kf = self.kb = 0
+        if int(history) < 0:
+            raise ValueError(f"history must not be negative, got {history}")
+        self.cache = CoefCache(sliced, self.lead, history, history_format, dev) if history else None
+        held = se.group_views(self.coef, self.lead, 1)
 
         def fwd_body(s0):
             self.win[:, :hop].copy_(self.win[:, hop:])
             self.win[:, hop:].copy_(self.chunk)
             se.analysis(self.win, 1, out=self.coef, slice0=s0, sample0=hop * (s0 - 1),
                         length=hop * (s0 + 1), ws=self.ws)
+            if self.cache is not None:
+                self.cache.append(*held)
 
         def bwd_body(s0):
             se.synthesis(self.cin, rows, 1, hop * (s0 + 1), out=self.ybuf, slice0=s0,
@@ -389,6 +406,16 @@ class SliceStream:
         self.win.zero_()
         self.tail.zero_()
         self.kf = self.kb = 0
+        if self.cache is not None:
+            self.cache.reset()
+
+    def past(self, n, dtype=torch.complex64, end=None):
+        """the last n slices that ``fwd`` / ``flush`` gave, from the history, as
+        (blocks [*lead, b, n * M], side [*lead, n, 1, M]); see
+        ``CoefCache.window``"""
+        if self.cache is None:
+            raise RuntimeError("this stream keeps no history (streamer(..., history=n))")
+        return self.cache.window(n, dtype=dtype, end=end)
 
     @staticmethod
     def _variant(k):
