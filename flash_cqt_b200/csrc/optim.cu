@@ -6,8 +6,8 @@
 //   m  = b1 m + (1 - b1) g'
 //   v  = b2 v + (1 - b2) g'^2
 //   p  = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
-// Each product and sum is rounded by itself (no fused multiply-add), so the
-// result does not depend on how a variant of the kernel is compiled.
+// Each product and sum of m and v is rounded by itself (no fused multiply-add),
+// so their bits do not depend on how a variant of the kernel is compiled.
 //
 // Moments in 8 bits: blocks of 256 elements (one warp, 8 elements a lane)
 // share a power-of-two scale per moment, one byte each.  m is held in e4m3, v
@@ -68,7 +68,9 @@ __host__ __device__ __forceinline__ unsigned mix32(unsigned x) {
     return x ^ (x >> 16);
 }
 
-// Two 32-bit floats in one instruction (sm_100), each rounded by itself.
+// Two 32-bit floats in one instruction (sm_100).  A product and a sum that takes
+// it may come out as one fused operation, so what has to have the bits of two
+// roundings is added with __fadd_rn.
 struct F2 {
     unsigned long long w;
 };
@@ -392,19 +394,24 @@ __device__ __forceinline__ void update8(const OptTensor& t, const Chunk<T, BITS,
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
         const F2 gi = two(g[i], g[i + 1]) * two(s.clip);
-        const F2 mi = two(m[i], m[i + 1]) + gi * two(a.omb1);
-        const F2 vi = two(v[i], v[i + 1]) + gi * gi * two(a.omb2);
+        // the sums one by one: a sum of packed products would be fused with
+        // them, and the moments' bits are those of separate roundings
+        float qa, qb, ra, rb;
+        split(gi * two(a.omb1), qa, qb);
+        m[i] = __fadd_rn(m[i], qa);
+        m[i + 1] = __fadd_rn(m[i + 1], qb);
+        split(gi * gi * two(a.omb2), ra, rb);
+        v[i] = __fadd_rn(v[i], ra);
+        v[i + 1] = __fadd_rn(v[i + 1], rb);
         // root and reciprocal to 2^-23: their last bits are far below the
         // parameter's own, and correctly rounded ones took a third of all
         // instructions.  2^-126 under the root keeps what is subnormal
         // from being read as 0 (above 2^-102 it changes nothing).
-        float ra, rb, da, db;
-        split(vi + two(0x1p-126f), ra, rb);
+        float da, db;
+        split(two(v[i], v[i + 1]) + two(0x1p-126f), ra, rb);
         split(two(root_of(ra), root_of(rb)) * two(s.root) + two(a.eps), da, db);
-        const F2 step = mi * two(one_over(da), one_over(db)) * two(-s.rate);
+        const F2 step = two(m[i], m[i + 1]) * two(one_over(da), one_over(db)) * two(-s.rate);
         split(two(p[i], p[i + 1]) * two(s.decay) + step, p[i], p[i + 1]);
-        split(mi, m[i], m[i + 1]);
-        split(vi, v[i], v[i + 1]);
     }
     uint2 mc, vc;
     int mk, vk;

@@ -143,6 +143,22 @@ def test_many_tensors(bits):
     assert abs(float(opt.grad_norm) - norm) <= norm * (po.U + 1e-12)
 
 
+def test_moments_have_the_bits_of_separate_roundings():
+    """m = fl(fl(b1 m) + fl((1 - b1) g)), v alike: nothing is fused"""
+    p = make([((4099,), torch.float32)], seed=20)[0]
+    opt = AdamW([p], lr=1e-3)
+    f = np.float32
+    m = v = np.zeros(4099, f)
+    for k in range(3):
+        p.grad = p.grad * 1.25 + 0.01 * k
+        g = p.grad.cpu().numpy()
+        opt.step()
+        m = m * f(0.9) + g * f(1 - 0.9)
+        v = v * f(0.999) + (g * g) * f(1 - 0.999)
+        assert np.array_equal(opt.state[p]["exp_avg"].cpu().numpy(), m)
+        assert np.array_equal(opt.state[p]["exp_avg_sq"].cpu().numpy(), v)
+
+
 def test_same_bits_every_time_and_across_lists():
     """no atomics order anything: two runs agree in every bit"""
     def run():
