@@ -459,18 +459,6 @@ __device__ __forceinline__ void update_part(const OptTensor& t, long long base, 
     update8(t, c, a, s, key, n, vec, ms, vs);
 }
 
-// the tensor that chunk c lies in: the last one whose first chunk is <= c
-template <int N>
-__device__ __forceinline__ int find_tensor(const OptTable<N>& tab, unsigned c) {
-    int lo = 0, hi = tab.count - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (tab.t[mid].chunk0 <= c) lo = mid;
-        else hi = mid - 1;
-    }
-    return lo;
-}
-
 constexpr int kWhole = 1 << 30;   // every thread has 8 aligned elements
 
 // the chunks of a tensor before this one have all their elements, aligned
@@ -479,14 +467,27 @@ __device__ __forceinline__ unsigned whole_end(const OptTensor& t) {
     return t.chunk0 + (t.vec == 2 ? (unsigned)(t.n / CHUNK) : 0);
 }
 
-// what the chunks need of their tensors is copied to shared memory first:
-// threads that look at different tensors would take turns at the parameters
-template <class Of>   // the first chunk of tensor i
-__device__ __forceinline__ int find_in(const Of& first, int count, unsigned c) {
+// The table rides in the kernel's parameters and is copied to shared memory with
+// ordinary loads, all of them at once: read as constants, 80 tensors' entries
+// miss the constant cache one after the other (10 us before the first chunk).
+template <int N>
+__device__ __forceinline__ void copy_table(const OptTable<N>& tab, OptTensor* to) {
+    static_assert(sizeof(OptTensor) % 8 == 0, "copied in words of 64 bits");
+    const unsigned long long* from = reinterpret_cast<const unsigned long long*>(tab.t);
+    unsigned long long* words = reinterpret_cast<unsigned long long*>(to);
+    for (int i = threadIdx.x; i < tab.count * (int)(sizeof(OptTensor) / 8); i += blockDim.x) {
+        unsigned long long w;
+        asm volatile("ld.u64 %0, [%1];" : "=l"(w) : "l"(from + i));
+        words[i] = w;
+    }
+}
+
+// the tensor that chunk c lies in: the last one whose first chunk is <= c
+__device__ __forceinline__ int find_tensor(const OptTensor* table, int count, unsigned c) {
     int lo = 0, hi = count - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (first(mid) <= c) lo = mid;
+        if (table[mid].chunk0 <= c) lo = mid;
         else hi = mid - 1;
     }
     return lo;
@@ -502,10 +503,10 @@ template <int N, class T, int BITS, bool MASTER>
 __global__ void __launch_bounds__(kStepThreads<BITS>, kStepCtas<BITS>)
 adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ OptArgs a) {
     constexpr int kThreads = kStepThreads<BITS>, kChunk = kThreads * kLane;
+    __shared__ __align__(8) OptTensor table[N];
     __shared__ TensorPlan tensor[N];
     __shared__ int chunk[kThreads];      // tensor of each of the CTA's next chunks, and kWhole
     __shared__ uint8_t scale[2][BITS == 8 ? kThreads * (kThreads / 32) : 1];
-    __shared__ unsigned whole[N];
     __shared__ long long steps[N];
     __shared__ StepScalars same;
     __shared__ unsigned order;
@@ -514,9 +515,11 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
     // what follows works out the scalars.
     Chunk<T, BITS, MASTER> here;
     const long long lane = threadIdx.x * kLane;
-    const int first = find_tensor(tab, blockIdx.x);
-    if (blockIdx.x < whole_end<kChunk>(tab.t[first]))
-        here.load(tab.t[first], (long long)(blockIdx.x - tab.t[first].chunk0) * kChunk + lane, 8, 2);
+    copy_table(tab, table);
+    __syncthreads();
+    const int first = find_tensor(table, tab.count, blockIdx.x);
+    if (blockIdx.x < whole_end<kChunk>(table[first]))
+        here.load(table[first], (long long)(blockIdx.x - table[first].chunk0) * kChunk + lane, 8, 2);
     if (threadIdx.x == kThreads - 1) {
         if (a.norm) pdl_wait();   // what else this kernel reads, the norm's does not write
         same.decay = (float)(1.0 - (a.lr_dev ? (double)*a.lr_dev : a.lr) * a.wd);
@@ -526,7 +529,7 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
     // 1 - b^t = -expm1(t ln b), which 32 bits hold to 2^-22 for every t
     const float lr = a.lr_dev ? *a.lr_dev : (float)a.lr;
     for (int i = threadIdx.x; i < tab.count; i += kThreads) {
-        const OptTensor& t = tab.t[i];
+        const OptTensor& t = table[i];
         const long long step = *t.step + 1;
         TensorPlan q;
         q.rate = lr / -expm1f((float)step * a.ln1);
@@ -534,7 +537,6 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
         q.key = BITS == 8 ? mix32(mix32(a.seed_key + (unsigned)step) + (unsigned)t.ordinal) : 0;
         q.chunk0 = t.chunk0;
         tensor[i] = q;
-        whole[i] = whole_end<kChunk>(t);
         steps[i] = step;
     }
     // tensors are looked up by one thread a chunk, a CTA's width at a time (the
@@ -547,8 +549,8 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
         __syncthreads();
         const unsigned long long mine = c0 + (unsigned long long)threadIdx.x * gridDim.x;
         if (mine < tab.chunks) {
-            const int i = find_in([&](int m) { return tensor[m].chunk0; }, tab.count, (unsigned)mine);
-            chunk[threadIdx.x] = i | ((unsigned)mine < whole[i] ? kWhole : 0);
+            const int i = find_tensor(table, tab.count, (unsigned)mine);
+            chunk[threadIdx.x] = i | ((unsigned)mine < whole_end<kChunk>(table[i]) ? kWhole : 0);
         }
         __syncthreads();
         const unsigned left = (tab.chunks - c0 - 1) / gridDim.x + 1;
@@ -557,7 +559,7 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
         const auto each_block = [&](auto f) {
             for (unsigned i = threadIdx.x; i < width * kWarps; i += kThreads) {
                 const unsigned k = i / kWarps, w = i - k * kWarps;
-                const OptTensor& t = tab.t[chunk[k] & ~kWhole];
+                const OptTensor& t = table[chunk[k] & ~kWhole];
                 const long long block = (long long)(c0 + k * gridDim.x - t.chunk0) * kWarps + w;
                 if (block * kOptBlock < t.n) f(i, t, block);
             }
@@ -573,7 +575,7 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
         unsigned c = c0;
         for (unsigned k = 0; k < width; ++k, c += gridDim.x) {
             const int i = chunk[k];
-            const OptTensor& t = tab.t[i & ~kWhole];
+            const OptTensor& t = table[i & ~kWhole];
             const TensorPlan q = tensor[i & ~kWhole];
             s.rate = q.rate;
             s.root = q.root;
@@ -581,7 +583,7 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
             const int j = more ? chunk[k + 1] : 0;
             Chunk<T, BITS, MASTER> next;
             if (j & kWhole) {
-                const OptTensor& u = tab.t[j & ~kWhole];
+                const OptTensor& u = table[j & ~kWhole];
                 next.load(u, (long long)(c + gridDim.x - u.chunk0) * kChunk + lane, 8, 2);
             }
             const long long base = (long long)(c - q.chunk0) * kChunk + lane;
@@ -605,7 +607,7 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
     if (threadIdx.x == 0) order = atomicAdd(a.ticket, 1u);
     __syncthreads();
     if (order != gridDim.x - 1) return;
-    for (int i = threadIdx.x; i < tab.count; i += kThreads) *tab.t[i].step = steps[i];
+    for (int i = threadIdx.x; i < tab.count; i += kThreads) *table[i].step = steps[i];
     if (threadIdx.x == 0) *a.ticket = 0;
 }
 
@@ -647,26 +649,23 @@ __global__ void __launch_bounds__(kNormThreads, kNormCtas / 148)
 norm_kernel(const __grid_constant__ OptTable<N> tab, double* partial, int first, int last,
             unsigned* ticket, double* norm, float* norm32) {
     constexpr int kChunk = kNormThreads * kLane;
-    __shared__ unsigned chunk0[N], whole[N];
+    __shared__ __align__(8) OptTensor table[N];
     __shared__ int tensor[kNormThreads];   // of each of the CTA's next chunks, and kWhole
     pdl_launch_dependents();
-    for (int i = threadIdx.x; i < tab.count; i += kNormThreads) {
-        chunk0[i] = tab.t[i].chunk0;
-        whole[i] = whole_end<kChunk>(tab.t[i]);
-    }
+    copy_table(tab, table);
     double part[4] = {0, 0, 0, 0};
     for (unsigned c0 = blockIdx.x; c0 < tab.chunks; c0 += kNormThreads * gridDim.x) {
         __syncthreads();
         const unsigned long long mine = c0 + (unsigned long long)threadIdx.x * gridDim.x;
         if (mine < tab.chunks) {
-            const int i = find_in([&](int m) { return chunk0[m]; }, tab.count, (unsigned)mine);
-            tensor[threadIdx.x] = i | ((unsigned)mine < whole[i] ? kWhole : 0);
+            const int i = find_tensor(table, tab.count, (unsigned)mine);
+            tensor[threadIdx.x] = i | ((unsigned)mine < whole_end<kChunk>(table[i]) ? kWhole : 0);
         }
         __syncthreads();
         unsigned c = c0;
         for (int k = 0; k < kNormThreads && c < tab.chunks; ++k, c += gridDim.x) {
             const int i = tensor[k];
-            const OptTensor& t = tab.t[i & ~kWhole];
+            const OptTensor& t = table[i & ~kWhole];
             const long long base = (long long)(c - t.chunk0) * kChunk + threadIdx.x * kLane;
             if (t.dtype == kOptF32) squares8<float>(t, base, i & kWhole, part);
             else if (t.dtype == kOptBf16) squares8<__nv_bfloat16>(t, base, i & kWhole, part);
