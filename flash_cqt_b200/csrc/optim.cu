@@ -37,15 +37,16 @@ namespace {
 
 constexpr int kLane = 8;                        // consecutive elements a thread
 static_assert(32 * kLane == kOptBlock, "a warp is one block");
-// CTA sizes.  Measured: 67 M float elements with 8-bit moments, 188 us with 4
-// CTAs of 224 threads an SM (72 registers), 188 with 3 of 256, 217 with 4 of 256
-// (64, some spilled); 96 M bf16 ones 219, 225 and 215 us.  32-bit moments move
-// more bytes an element and want fewer threads: 144 M bf16 elements with a master
-// copy 660 us with 16 warps an SM, 675 with 24, 750 with 32.
+// CTA sizes.  Measured with 8-bit moments, 67 M float and 96 M bf16 elements: 181
+// and 225 us with 7 CTAs of 128 threads an SM (72 registers), 190 and 233 with 3
+// of 256, 192 and 233 with 4 of 192, 210 and 224 with 4 of 224, 221 and 315 with
+// 4 of 256 (64 registers, spilled).  32-bit moments move more bytes an element
+// and want fewer threads: 144 M bf16 elements with a master copy 660 us with 16
+// warps an SM, 675 with 24, 750 with 32.
 template <int BITS>
-constexpr int kStepThreads = BITS == 8 ? 224 : 256;
+constexpr int kStepThreads = BITS == 8 ? 128 : 256;
 template <int BITS>
-constexpr int kStepCtas = BITS == 8 ? 4 : 2;    // of an SM
+constexpr int kStepCtas = BITS == 8 ? 7 : 2;    // of an SM
 constexpr int kNormThreads = 256;
 
 template <int N>
