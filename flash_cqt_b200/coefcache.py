@@ -148,7 +148,7 @@ class CoefCache:
         parts = (_native.CqtCachePart * len(self.gspec))()
         keep = []
         for k, (c, (b, M)) in enumerate(zip(blocks + side, self.gspec)):
-            c = c.resolve_conj()
+            c = c.resolve_conj().resolve_neg()
             v = c.reshape(self.rows, b, S * M) if k < self.ngroups else c.reshape(self.rows, S, b, M)
             if (v.stride(-1) != 1 and v.shape[-1] > 1) or v.data_ptr() % 8:
                 v = v.clone(memory_format=torch.contiguous_format)

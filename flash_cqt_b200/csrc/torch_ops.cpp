@@ -779,7 +779,7 @@ struct CacheHandle {
         for (size_t k = 0; k < all.size(); ++k) {
             const at::Tensor& c = all[k];
             if (!c.defined() || !c.is_cuda() || c.get_device() != device ||
-                c.scalar_type() != at::kComplexFloat || c.is_conj())
+                c.scalar_type() != at::kComplexFloat || c.is_conj() || c.is_neg())
                 return false;
             const bool side = (int64_t)k >= ngroups;
             const int64_t b = bands[k], M = lens[k];

@@ -89,8 +89,9 @@ class AdamW(torch.optim.Optimizer):
 
     Steps of one optimizer must be ordered on one stream at a time.  State is
     made at a parameter's first step; before a step is captured it has to be
-    there (``init_state()``, or a step).  State is replaced through
-    ``load_state_dict`` (which also takes the state of ``torch.optim.AdamW``).
+    there (``init_state()``, or a step).  ``load_state_dict`` (which also takes the
+    state of ``torch.optim.AdamW``) writes into the state that is there, so a
+    captured step goes on from what was loaded.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *,
@@ -112,7 +113,8 @@ class AdamW(torch.optim.Optimizer):
 
     def __setstate__(self, state):
         super().__setstate__(state)
-        self._reset()
+        if "_retired" not in self.__dict__:   # a new object (load_state_dict comes here too)
+            self._reset()
         for g in self.param_groups:
             self._dev = g["params"][0].device if g["params"] else self._dev
         self._total = sum(len(g["params"]) for g in self.param_groups)
@@ -138,6 +140,8 @@ class AdamW(torch.optim.Optimizer):
     def add_param_group(self, group):
         group = dict(group)
         params = group["params"]
+        if isinstance(params, (set, frozenset)):
+            raise TypeError("parameters must be in an order of their own: a set has none")
         params = [params] if torch.is_tensor(params) else list(params)
         group["params"] = params
         self._check_options({**self.defaults, **group})
@@ -231,10 +235,12 @@ class AdamW(torch.optim.Optimizer):
                 if not self.state.get(p):
                     self.state[p] = self._new_state(p, g)
 
+    @torch.no_grad()
     def load_state_dict(self, state_dict):
         state_dict = dict(state_dict)
         saved = state_dict["state"]
         groups = state_dict["param_groups"]
+        before = dict(self.state)
         # the base class would cast the state to the parameters' types: it
         # only takes the groups, the state is laid out here
         super().load_state_dict(dict(state_dict, state={}))
@@ -258,6 +264,12 @@ class AdamW(torch.optim.Optimizer):
                 if g["master"] and "master" not in s and p.dtype in (torch.bfloat16, torch.float16):
                     s["master"] = p.detach().float()
                 self._check_state(s, p, g)
+                # into the tensors that are there: a captured step goes on with them
+                for k, v in s.items():
+                    at = before.get(p, {}).get(k)
+                    if torch.is_tensor(at) and at.dtype == v.dtype and at.shape == v.shape \
+                            and at.device == v.device and at.stride() == v.stride():
+                        s[k] = at.copy_(v)
                 new[p] = s
         self.state.clear()
         self.state.update(new)

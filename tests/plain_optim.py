@@ -46,12 +46,12 @@ def _mix(x):
     return x ^ (x >> np.uint32(16))
 
 
-def noise(seed, t, ordinal, n):
-    """32 random bits for every element"""
+def noise(seed, t, ordinal, n, start=0):
+    """32 random bits for every element from number `start` on"""
     w = np.uint64(0xffffffff)
     add = lambda a, b: np.uint32((np.uint64(a) + np.uint64(b)) & w)  # noqa: E731
     key = _mix(add(_mix(add(_mix(np.uint32(seed)), t)), ordinal))
-    i = np.arange(n, dtype=np.uint64)
+    i = np.arange(start, start + n, dtype=np.uint64)
     key = _mix(((np.uint64(key) + (i >> np.uint64(32))) & w).astype(np.uint32))
     return _mix((i & w).astype(np.uint32) ^ key)
 

@@ -60,12 +60,11 @@ def same(a, b):
 
 
 def check_store(cache, ring):
-    rows, cap = ring.codes.shape[:2]
-    c = cache.codes.double().cpu().numpy().reshape(rows, cap, -1)
+    c = cache.codes.double().cpu().numpy().reshape(ring.codes.shape)
     if cache.fmt == "int8":
         c = np.where(c == -128, np.nan, c)
     assert same(c, ring.codes)
-    assert same(cache.scales.double().cpu().numpy().reshape(rows, cap, -1), ring.scales)
+    assert same(cache.scales.double().cpu().numpy().reshape(ring.scales.shape), ring.scales)
     assert same(cache.length.cpu().numpy().reshape(-1), ring.length)
 
 
@@ -148,12 +147,54 @@ def test_views_and_orders(banks):
     assert all(b.data_ptr() % 16 == 8 for b in longer)
     swapped = [b.transpose(1, 2).contiguous().transpose(1, 2) for b in blocks]
     lazy = [b.conj().resolve_conj().conj() for b in blocks]
+    negated = [torch._neg_view(-b) for b in blocks]
     rows = [torch.stack([b, b], 1)[:, 1] for b in blocks]
-    for v in (longer, swapped, lazy, rows):
+    assert negated[0].is_neg()
+    for v in (longer, swapped, lazy, negated, rows):
         cache = CoefCache(cqt, (2,), 4, device=DEV)
         cache.append(v, [s.transpose(0, 1).contiguous().transpose(0, 1) for s in side])
         check_store(cache, ring)
     assert lazy[0].is_conj()
+
+
+@pytest.mark.parametrize("lead", [(), (0,), (2, 0), (3,), (2, 1, 2)])
+def test_leading_dimensions(banks, lead):
+    """no dimensions, no streams, several dimensions"""
+    cqt = banks["short"]
+    rows = int(np.prod(lead))
+    cache, ring = CoefCache(cqt, lead, 2, device=DEV), pc.Ring(rows, 2, cqt.heap.ncoef, "int8")
+    for seed in range(3):
+        h = heaps(rows, 1, cqt.heap.ncoef, seed)
+        cache.append(*to_blocks(h, cqt, lead))
+        ring.append(h)
+    check_store(cache, ring)
+    b, s = cache.window(3)
+    assert b[0].shape[:len(lead)] == lead and s[0].shape[len(lead)] == 3
+    assert same(from_blocks(b, s, cqt, 3), ring.window(3))
+
+
+def test_many_slices_and_streams(banks):
+    """more streams, and more slices, than a grid's extents hold"""
+    cqt = banks["short"]
+    nc = cqt.heap.ncoef
+    h = heaps(1, 1, nc, 0)
+    b, s = to_blocks(h, cqt, (1,))
+    rows = 65537
+    cache = CoefCache(cqt, (rows,), 1, device=DEV)
+    cache.append([x.expand(rows, *x.shape[1:]) for x in b], [x.expand(rows, *x.shape[1:]) for x in s])
+    assert (cache.length == 1).all()
+    assert torch.equal(cache.codes[0], cache.codes[rows - 1])
+    assert (cache.codes[::8191] == cache.codes[:1]).all()
+    ring = pc.Ring(1, 1, nc, "int8")
+    ring.append(h)
+    assert same(cache.codes[rows - 1].double().cpu().numpy().reshape(1, 1, -1), ring.codes)
+    # a window far longer than the ring: zeros but for its end
+    one = CoefCache(cqt, (1,), 1, device=DEV)
+    one.append(b, s)
+    blocks, _ = one.window(65540, dtype=torch.bfloat16)
+    M = cqt.heap.gspec[0][1]
+    assert same(blocks[0][0, 0, -M:].double().cpu().numpy(), ring.window(1)[0, 0, :M])
+    assert not blocks[0][0, 0, :-M].any() and not blocks[5][0, :, :M].any()
 
 
 def test_rows_left_alone(banks):

@@ -536,12 +536,83 @@ def test_deepcopy_and_save():
     assert torch.equal(p, q2)
 
 
+def test_load_into_a_captured_step():
+    """a captured step goes on from a state that is loaded later"""
+    def setup():
+        p = make([((600,), torch.float32)], seed=21)[0]
+        return p, AdamW([p], lr=1e-2, state_bits=8, max_norm=0.5)
+    p, opt = setup()
+    q, ref = setup()
+    for _ in range(2):
+        ref.step()
+    saved = copy.deepcopy(ref.state_dict())
+    opt.init_state()
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    opt.load_state_dict(saved)
+    with torch.no_grad():
+        p.copy_(q)
+    graph.replay()
+    ref.step()
+    assert torch.equal(p, q) and int(opt.state[p]["step"]) == 3
+
+
+def test_first_step_of_a_process_in_a_capture():
+    """nothing that has to happen outside of a capture is left to a first launch"""
+    import subprocess
+    import sys
+    code = """
+import torch
+from flash_cqt_b200 import AdamW
+p = torch.ones(1000, device="cuda", requires_grad=True)
+p.grad = torch.ones_like(p)
+opt = AdamW([p], lr=0.5, weight_decay=0.0, state_bits=8, max_norm=1e9)
+opt.init_state()
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    opt.step()
+g.replay()
+torch.cuda.synchronize()
+assert abs(float(p[0]) - 0.5) < 1e-5 and int(opt.state[p]["step"]) == 1
+print("fine")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
+
+
+def test_more_than_2_32_elements():
+    """offsets and noise beyond 32 bits"""
+    far, tail = 2 ** 32, 3001
+    p = torch.zeros(far + tail, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    p.grad = torch.zeros(far + tail, dtype=torch.bfloat16, device=DEV)
+    p.grad[-tail:] = torch.randn(tail, device=DEV)
+    p.grad[:5] = 1.0
+    g = p.grad[-tail:].double().cpu().numpy()
+    opt = AdamW([p], lr=1e-2, weight_decay=0.0, state_bits=8, max_norm=1e3, seed=4)
+    opt.step()
+    assert abs(float(opt.grad_norm) - np.sqrt((g ** 2).sum() + 5)) <= float(opt.grad_norm) * po.U * 1.01
+    z = np.zeros(tail)
+    p1, m1, _, (ep, em, _) = po.step(z, g, z, z, 1, 1e-2, 0.9, 0.999, 1e-8, 0.0)
+    assert np.all(np.abs(flat(p[-tail:]) - p1) <= ep + 2.0 ** -8 * (np.abs(p1) + ep))
+    s = opt.state[p]
+    sc = s["exp_avg_scale"][far // 256:].double().cpu().numpy()
+    got = s["exp_avg"][-tail:].double().cpu().numpy() * po.spread(sc, tail)
+    h = po.noise(4, 1, 0, tail, start=far)
+    assert np.all((po.round_m(m1 - em, sc, h) <= got) & (got <= po.round_m(m1 + em, sc, h)))
+    assert float(s["exp_avg"][5:4096].float().abs().max()) == 0 and float(p[:5].float().max()) < 0
+
+
 def test_refusals():
     p = torch.zeros(8, device=DEV, requires_grad=True)
     with pytest.raises(ValueError, match="share memory"):
         AdamW([p, p.detach()[2:4].requires_grad_()])
     with pytest.raises(ValueError, match="share memory"):
         AdamW([p, p])
+    with pytest.raises(TypeError, match="set"):
+        AdamW([dict(params={p})])
     opt = AdamW([p])
     with pytest.raises(ValueError, match="share memory"):
         opt.add_param_group(dict(params=[p]))
