@@ -138,30 +138,41 @@ __device__ __forceinline__ uint4 encode(const float (&x)[16], float peak, int& e
     return make_uint4(c[0], c[1], c[2], c[3]);
 }
 
-// 4 codes to values
+// 16 codes to values
 template <bool INT8>
-__device__ __forceinline__ void decode(unsigned w, uint8_t e, float (&x)[4]) {
+__device__ __forceinline__ void decode(uint4 c, uint8_t e, float (&x)[16]) {
     const float s = __uint_as_float(e ? (unsigned)e << 23 : 0x400000u);
+    const unsigned w[4] = {c.x, c.y, c.z, c.w};
     if constexpr (INT8) {
-        const unsigned u = w ^ 0x80808080u;   // the codes plus 128
-        // a byte of 0 is the code of NaN; and the one product and sum below
-        // need (2^23 + 128) s to be finite
-        const bool rare = ((u - 0x01010101u) & ~u & 0x80808080u) != 0 || e > 200;
+        unsigned nan = 0;
         const float off = -8388736.f * s;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float f = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 | k));   // 2^23 + byte
-            x[k] = fmaf(f, s, off);
-            if (rare) x[k] = f == 8388608.f ? __int_as_float(0x7fffffff) : (f - 8388736.f) * s;
+        for (int i = 0; i < 4; ++i) {
+            const unsigned u = w[i] ^ 0x80808080u;   // the codes plus 128
+            nan |= (u - 0x01010101u) & ~u;           // bit 7 of a byte that is 0, the code of NaN
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                // 2^23 + byte, less 2^23 + 128, times s, rounded once (exactly)
+                const float f = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 | k));
+                x[4 * i + k] = fmaf(f, s, off);
+            }
+        }
+        // that needs (2^23 + 128) s to be finite
+        if ((nan & 0x80808080u) != 0 || e > 200) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int code = (int)(w[i / 4] << (24 - 8 * (i & 3))) >> 24;
+                x[i] = code == -128 ? __int_as_float(0x7fffffff) : (float)code * s;
+            }
         }
     } else {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+        for (int i = 0; i < 8; ++i) {
             const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(
-                (__nv_fp8x2_storage_t)(k ? w >> 16 : w & 0xffffu), __NV_E4M3);
+                (__nv_fp8x2_storage_t)((i & 1) ? w[i / 2] >> 16 : w[i / 2] & 0xffffu), __NV_E4M3);
             const float2 f = __half22float2(__half2(h));
-            x[2 * k] = f.x * s;
-            x[2 * k + 1] = f.y * s;
+            x[2 * i] = f.x * s;
+            x[2 * i + 1] = f.y * s;
         }
     }
 }
@@ -327,15 +338,8 @@ window_kernel(const __grid_constant__ CacheStore st, const __grid_constant__ Cac
                 const int q = blockIdx.x * kTile + i * kThreads + threadIdx.x;
                 if (q >= octs) continue;
                 T* dst = reinterpret_cast<T*>(place(gr, sb, item, 8 * q));
-                const unsigned w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
                 float y[16];
-#pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    float a[4];
-                    decode<INT8>(w[h], e[i], a);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) y[4 * h + k] = a[k];
-                }
+                decode<INT8>(c[i], e[i], y);
                 store16(dst, gr.wide, y);
             }
         }
