@@ -463,9 +463,8 @@ __device__ __forceinline__ void update_part(const OptTensor& t, long long base, 
 constexpr int kWhole = 1 << 30;   // every thread has 8 aligned elements
 
 // the chunks of a tensor before this one have all their elements, aligned
-template <int CHUNK>
-__device__ __forceinline__ unsigned whole_end(const OptTensor& t) {
-    return t.chunk0 + (t.vec == 2 ? (unsigned)(t.n / CHUNK) : 0);
+__device__ __forceinline__ unsigned whole_end(const OptTensor& t, int chunk) {
+    return t.chunk0 + (t.vec == 2 ? (unsigned)(t.n / chunk) : 0);
 }
 
 // The table rides in the kernel's parameters and is copied to shared memory with
@@ -519,7 +518,7 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
     copy_table(tab, table);
     __syncthreads();
     const int first = find_tensor(table, tab.count, blockIdx.x);
-    if (blockIdx.x < whole_end<kChunk>(table[first]))
+    if (blockIdx.x < whole_end(table[first], kChunk))
         here.load(table[first], (long long)(blockIdx.x - table[first].chunk0) * kChunk + lane, 8, 2);
     if (threadIdx.x == kThreads - 1) {
         if (a.norm) pdl_wait();   // what else this kernel reads, the norm's does not write
@@ -551,7 +550,7 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
         const unsigned long long mine = c0 + (unsigned long long)threadIdx.x * gridDim.x;
         if (mine < tab.chunks) {
             const int i = find_tensor(table, tab.count, (unsigned)mine);
-            chunk[threadIdx.x] = i | ((unsigned)mine < whole_end<kChunk>(table[i]) ? kWhole : 0);
+            chunk[threadIdx.x] = i | ((unsigned)mine < whole_end(table[i], kChunk) ? kWhole : 0);
         }
         __syncthreads();
         const unsigned left = (tab.chunks - c0 - 1) / gridDim.x + 1;
@@ -614,23 +613,49 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
 
 // ---- sqrt(sum of squares over all gradients), summed in 64 bits in a fixed
 // order: threads, warps, CTAs, launches
-// a thread's 8 elements of a chunk, some of them or none
+
+// elements of a chunk: 32 bytes a thread, so that 16-bit gradients have as many
+// bytes on their way as 32-bit ones
+__host__ __device__ constexpr int norm_chunk(int dtype) {
+    return kNormThreads * (dtype == kOptF32 ? 8 : 16);
+}
+
+__device__ __forceinline__ void add_square(float x, double& sum) {
+    sum = fma((double)x, (double)x, sum);
+}
+
+// a thread's elements of chunk `chunk` of a tensor, some of them or none
 template <class T>
-__device__ __forceinline__ void squares8(const OptTensor& t, long long base, bool whole,
-                                         double (&sum)[4]) {
+__device__ __forceinline__ void squares(const OptTensor& t, long long chunk, bool whole,
+                                        double (&sum)[4]) {
+    constexpr int kEach = 32 / sizeof(T);
+    const long long base = (chunk * kNormThreads + threadIdx.x) * kEach;
     const T* g = static_cast<const T*>(t.g) + base;
-    Raw8<T> r;
     if (whole) {
-        load8(g, 2, 8, r);
-    } else {
-        const long long left = t.n - base;
-        const int n = left >= 8 ? 8 : (left > 0 ? (int)left : 0);
-        load8(g, n == 8 ? t.vec : 0, n, r);
-    }
-    float x[8];
-    unpack(r, x);
+        float w[8];
+        load_v8(reinterpret_cast<const float*>(g), w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum[i & 3] = fma((double)x[i], (double)x[i], sum[i & 3]);
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                add_square(w[i], sum[i & 3]);
+            } else {
+                const float2 f = pair_to_float<T>(__float_as_uint(w[i]));
+                add_square(f.x, sum[i & 1]);
+                add_square(f.y, sum[2 + (i & 1)]);
+            }
+        }
+    } else {
+        for (int k = 0; k < kEach; k += 8) {
+            const long long left = t.n - base - k;
+            const int n = left >= 8 ? 8 : (left > 0 ? (int)left : 0);
+            Raw8<T> r;
+            float x[8];
+            load8(g + k, n == 8 ? t.vec : 0, n, r);
+            unpack(r, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) add_square(x[i], sum[i & 3]);
+        }
+    }
 }
 
 __device__ __forceinline__ double cta_sum(double x) {
@@ -649,7 +674,6 @@ template <int N>
 __global__ void __launch_bounds__(kNormThreads, kNormCtas / 148)
 norm_kernel(const __grid_constant__ OptTable<N> tab, double* partial, int first, int last,
             unsigned* ticket, double* norm, float* norm32) {
-    constexpr int kChunk = kNormThreads * kLane;
     __shared__ __align__(8) OptTensor table[N];
     __shared__ int tensor[kNormThreads];   // of each of the CTA's next chunks, and kWhole
     pdl_launch_dependents();
@@ -660,17 +684,17 @@ norm_kernel(const __grid_constant__ OptTable<N> tab, double* partial, int first,
         const unsigned long long mine = c0 + (unsigned long long)threadIdx.x * gridDim.x;
         if (mine < tab.chunks) {
             const int i = find_tensor(table, tab.count, (unsigned)mine);
-            tensor[threadIdx.x] = i | ((unsigned)mine < whole_end<kChunk>(table[i]) ? kWhole : 0);
+            tensor[threadIdx.x] = i | ((unsigned)mine < whole_end(table[i], norm_chunk(table[i].dtype)) ? kWhole : 0);
         }
         __syncthreads();
         unsigned c = c0;
         for (int k = 0; k < kNormThreads && c < tab.chunks; ++k, c += gridDim.x) {
             const int i = tensor[k];
             const OptTensor& t = table[i & ~kWhole];
-            const long long base = (long long)(c - t.chunk0) * kChunk + threadIdx.x * kLane;
-            if (t.dtype == kOptF32) squares8<float>(t, base, i & kWhole, part);
-            else if (t.dtype == kOptBf16) squares8<__nv_bfloat16>(t, base, i & kWhole, part);
-            else squares8<__half>(t, base, i & kWhole, part);
+            const long long at = (long long)(c - t.chunk0);
+            if (t.dtype == kOptF32) squares<float>(t, at, i & kWhole, part);
+            else if (t.dtype == kOptBf16) squares<__nv_bfloat16>(t, at, i & kWhole, part);
+            else squares<__half>(t, at, i & kWhole, part);
         }
     }
     double sum = (part[0] + part[1]) + (part[2] + part[3]);
@@ -702,10 +726,11 @@ unsigned opt_grid(unsigned chunks, unsigned most) {
 }
 
 template <int N>
-void fill(OptTable<N>* tab, const OptTensor* t, int count, int chunk) {
+void fill(OptTable<N>* tab, const OptTensor* t, int count, int chunk_of) {
     tab->count = count;
     unsigned c = 0;
     for (int i = 0; i < count; ++i) {
+        const int chunk = chunk_of ? chunk_of : norm_chunk(t[i].dtype);   // 0: the norm's
         tab->t[i] = t[i];
         tab->t[i].chunk0 = c;
         c += (unsigned)((t[i].n + chunk - 1) / chunk);
@@ -758,7 +783,7 @@ template <int N>
 cudaError_t norm_part(const OptTensor* t, int count, double* partial, int* first, bool last,
                       unsigned* ticket, double* norm, float* norm32, cudaStream_t s) {
     OptTable<N> tab;
-    fill(&tab, t, count, kNormThreads * kLane);
+    fill(&tab, t, count, 0);
     const unsigned grid = opt_grid(tab.chunks, kNormCtas);
     norm_kernel<N><<<grid, kNormThreads, 0, s>>>(tab, partial, *first, last ? 1 : 0, ticket, norm,
                                              norm32);
