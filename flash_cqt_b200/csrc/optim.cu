@@ -21,6 +21,11 @@
 //
 // The table of tensors rides in the kernel parameters (up to 32 KB): no copy
 // before the launch, and a captured graph holds it.
+//
+// Every byte is touched once, so DRAM bounds the step: 144 M bf16 elements with
+// a master copy 660 us (6.1 TB/s), 67 M floats with 8-bit moments 180 us (6.0
+// TB/s).  16-bit parameters with 8-bit moments move 10 bytes for 57 instructions
+// an element and stay at 4.3 TB/s (96 M elements, 225 us).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -612,7 +617,8 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
 }
 
 // ---- sqrt(sum of squares over all gradients), summed in 64 bits in a fixed
-// order: threads, warps, CTAs, launches
+// order: threads, warps, CTAs, launches.  Bound by what its start and its end cost
+// and by loads on their way: 210 MB take 46 us (4.6 TB/s), 50 MB 16, nothing 4.
 
 // elements of a chunk: 32 bytes a thread, so that 16-bit gradients have as many
 // bytes on their way as 32-bit ones
