@@ -507,6 +507,11 @@ struct AdamWPlan {
     std::vector<int64_t> ends;           // of each group in todo
     std::vector<at::Tensor> keep;
 
+    static int32_t type_of(const at::Tensor& p) {
+        return p.scalar_type() == at::kBFloat16 ? CQT_BF16
+               : p.scalar_type() == at::kHalf   ? CQT_F16
+               : p.scalar_type() == at::kFloat || p.scalar_type() == at::kComplexFloat ? CQT_F32 : -1;
+    }
     static void walk(PyObject* state, std::vector<PyObject*>& out) {
         PyObject *k, *v;
         Py_ssize_t at = 0;
@@ -541,8 +546,7 @@ struct AdamWPlan {
                 s.p = p.cast<at::Tensor>();
                 s.d.ordinal = ordinal++;
                 s.d.numel = s.p.numel() * (s.p.is_complex() ? 2 : 1);
-                s.d.dtype = s.p.scalar_type() == at::kBFloat16 ? CQT_BF16
-                            : s.p.scalar_type() == at::kHalf   ? CQT_F16 : CQT_F32;
+                s.d.dtype = type_of(s.p);
                 pybind11::object mine = pybind11::none();
                 if (state.contains(p)) mine = state[p];
                 if (!pybind11::isinstance<pybind11::dict>(mine)) continue;
@@ -613,7 +617,8 @@ struct AdamWPlan {
                                   " on ", grad.device());
                 // the parameter's storage may have been exchanged
                 const int64_t n = p.numel() * (p.is_complex() ? 2 : 1);
-                if (n != s.d.numel || !p.is_non_overlapping_and_dense() || p.get_device() != device)
+                if (n != s.d.numel || type_of(p) != s.d.dtype || p.get_device() != device ||
+                    !p.is_non_overlapping_and_dense() || p.is_conj() || p.is_neg())
                     return false;
                 if (g.bits == 32 && (s.m.sizes() != p.sizes() || !same_order(s.m, p) ||
                                      s.v.sizes() != p.sizes() || !same_order(s.v, p)))
@@ -663,49 +668,52 @@ struct AdamWPlan {
         auto check = [&](int rc, const char* what) {
             TORCH_CHECK(rc == 0, what, " failed (", rc, "): ", last_error());
         };
-        cqt_adamw_args a{};
-        a.use_norm = max_norm.is_none() ? 0 : 2;   // 1 after the first launch behind the norm
-        a.max_norm = a.use_norm ? number(max_norm.ptr()) : 0.0;
-        a.seed = seed;
-        if (a.use_norm)
-            check(norm_fn(todo.data(), (int)todo.size(), norm->data_ptr<float>(), ws.data_ptr(),
-                          (size_t)ws.numel(), stream),
-                  "cqt_grad_norm");
-        int64_t first = 0;
-        size_t k = 0;
+        // all options are read and checked before anything is changed
+        std::vector<cqt_adamw_args> args;
+        int use_norm = max_norm.is_none() ? 0 : 2;   // 1 after the launch behind the norm
         for (auto gr : param_groups) {
-            const int64_t last = ends[k];
-            const int bits = groups[k++].bits;
-            if (last == first) continue;
             PyObject* g = gr.ptr();
             PyObject* lr = item(g, "lr");
-            PyObject* betas = item(g, "betas");
-            if (THPVariable_Check(lr)) {
+            cqt_adamw_args a{};
+            a.max_norm = use_norm ? number(max_norm.ptr()) : 0.0;
+            a.seed = seed;
+            if (THPVariable_Check(lr) && THPVariable_Unpack(lr).is_cuda()) {
                 const at::Tensor& t = THPVariable_Unpack(lr);
-                if (t.is_cuda()) {
-                    TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat, "a device lr must be float32, got ",
-                                     t.scalar_type());
-                    TORCH_CHECK_VALUE(t.numel() == 1 && t.get_device() == device,
-                                      "a device lr must hold one number on cuda:", (int)device);
-                    a.lr_dev = t.data_ptr<float>();
-                    a.lr = 0;
-                } else {
-                    a.lr_dev = nullptr;
-                    a.lr = t.item<double>();
-                }
+                TORCH_CHECK_TYPE(t.scalar_type() == at::kFloat, "a device lr must be float32, got ",
+                                 t.scalar_type());
+                TORCH_CHECK_VALUE(t.numel() == 1 && t.get_device() == device,
+                                  "a device lr must hold one number on cuda:", (int)device);
+                a.lr_dev = t.data_ptr<float>();
             } else {
-                a.lr_dev = nullptr;
-                a.lr = number(lr);
+                a.lr = THPVariable_Check(lr) ? THPVariable_Unpack(lr).item<double>() : number(lr);
             }
-            pybind11::sequence bs = pybind11::reinterpret_borrow<pybind11::sequence>(betas);
+            pybind11::sequence bs = pybind11::reinterpret_borrow<pybind11::sequence>(item(g, "betas"));
             a.beta1 = bs[0].cast<double>();
             a.beta2 = bs[1].cast<double>();
             a.eps = number(item(g, "eps"));
             a.weight_decay = number(item(g, "weight_decay"));
-            check(step_fn(todo.data() + first, (int)(last - first), bits, &a, ws.data_ptr(),
+            TORCH_CHECK_VALUE(a.lr >= 0, "lr must not be negative, got ", a.lr);
+            TORCH_CHECK_VALUE(a.beta1 >= 0 && a.beta1 < 1 && a.beta2 >= 0 && a.beta2 < 1,
+                              "betas must lie in [0, 1), got ", a.beta1, ", ", a.beta2);
+            TORCH_CHECK_VALUE(a.eps >= 0 && a.weight_decay >= 0,
+                              "eps and weight_decay must not be negative");
+            args.push_back(a);
+        }
+        if (use_norm) {
+            TORCH_CHECK_VALUE(args.empty() || args[0].max_norm > 0, "max_norm must be positive");
+            check(norm_fn(todo.data(), (int)todo.size(), norm->data_ptr<float>(), ws.data_ptr(),
                           (size_t)ws.numel(), stream),
+                  "cqt_grad_norm");
+        }
+        int64_t first = 0;
+        for (size_t k = 0; k < args.size(); ++k) {
+            const int64_t last = ends[k];
+            if (last == first) continue;
+            args[k].use_norm = use_norm;
+            check(step_fn(todo.data() + first, (int)(last - first), groups[k].bits, &args[k],
+                          ws.data_ptr(), (size_t)ws.numel(), stream),
                   "cqt_adamw_step");
-            if (a.use_norm) a.use_norm = 1;
+            if (use_norm) use_norm = 1;
             first = last;
         }
         keep.clear();

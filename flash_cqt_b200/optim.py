@@ -237,42 +237,54 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def load_state_dict(self, state_dict):
-        state_dict = dict(state_dict)
-        saved = state_dict["state"]
+        """take over the options and the state of ``state_dict``; on a state that
+        does not fit, ValueError, and the optimizer is as it was"""
         groups = state_dict["param_groups"]
-        before = dict(self.state)
-        # the base class would cast the state to the parameters' types: it
-        # only takes the groups, the state is laid out here
-        super().load_state_dict(dict(state_dict, state={}))
-        for g in self.param_groups:
-            for k, v in self.defaults.items():
-                g.setdefault(k, v)
-        new = {}
-        for old, g in zip(groups, self.param_groups):
-            for i, p in zip(old["params"], g["params"]):
-                if not saved.get(i):
-                    continue
-                s = {}
-                for k, v in saved[i].items():
-                    if k == "step":
-                        s[k] = torch.as_tensor(v).detach().to(p.device, torch.int64).reshape(()).clone()
-                    elif torch.is_tensor(v):
-                        v = v.detach().to(p.device, copy=True)
-                        if v.shape == p.shape and not _same_order(v, p):
-                            v = torch.empty_like(p, dtype=v.dtype, requires_grad=False).copy_(v)
-                        s[k] = v
-                if g["master"] and "master" not in s and p.dtype in (torch.bfloat16, torch.float16):
-                    s["master"] = p.detach().float()
-                self._check_state(s, p, g)
-                # into the tensors that are there: a captured step goes on with them
-                for k, v in s.items():
-                    at = before.get(p, {}).get(k)
-                    if torch.is_tensor(at) and at.dtype == v.dtype and at.shape == v.shape \
-                            and at.device == v.device and at.stride() == v.stride():
-                        s[k] = at.copy_(v)
-                new[p] = s
+        if any(g.get("amsgrad") or g.get("maximize") for g in groups):
+            raise ValueError("amsgrad and maximize do not exist here")
+        before, was = dict(self.state), [dict(g) for g in self.param_groups]
+        try:
+            # the base class would cast the state to the parameters' types: it
+            # only takes the groups, the state is laid out here
+            super().load_state_dict(dict(state_dict, state={}))
+            for g in self.param_groups:
+                for k, v in self.defaults.items():
+                    g.setdefault(k, v)
+            new = {p: self._loaded(state_dict["state"][i], p, g)
+                   for old, g in zip(groups, self.param_groups)
+                   for i, p in zip(old["params"], g["params"]) if state_dict["state"].get(i)}
+        except Exception:
+            self.param_groups[:] = was
+            self.state.clear()
+            self.state.update(before)
+            raise
+        for p, s in new.items():
+            # into the tensors that are there: a captured step goes on with them
+            for k, v in s.items():
+                at = before.get(p, {}).get(k)
+                if torch.is_tensor(at) and at.dtype == v.dtype and at.shape == v.shape \
+                        and at.device == v.device and at.stride() == v.stride():
+                    s[k] = at.copy_(v)
         self.state.clear()
         self.state.update(new)
+
+    def _loaded(self, saved, p, g):
+        """a parameter's saved state as new tensors, laid out for the kernels"""
+        s = {}
+        for k, v in saved.items():
+            if k == "step":
+                s[k] = torch.as_tensor(v).detach().to(p.device, torch.int64).reshape(()).clone()
+            elif torch.is_tensor(v):
+                v = v.detach().to(p.device, copy=True)
+                if g["state_bits"] == 32 and v.dtype in (torch.bfloat16, torch.float16):
+                    v = v.float()   # moments that were kept in the parameter's type
+                if v.shape == p.shape and not _same_order(v, p):
+                    v = torch.empty_like(p, dtype=v.dtype, requires_grad=False).copy_(v)
+                s[k] = v
+        if g["master"] and "master" not in s and p.dtype in (torch.bfloat16, torch.float16):
+            s["master"] = p.detach().float()
+        self._check_state(s, p, g)
+        return s
 
     # -------------------------------------------------------------------- step
     def _grad(self, p):

@@ -384,6 +384,43 @@ def test_state_of_torch_adamw():
     check_step(b, qs, 2, kw)
 
 
+def test_refused_state_changes_nothing():
+    p, q = make([((40,), torch.float32), ((30,), torch.float32)], seed=22)
+    opt = AdamW([p, q], lr=1e-2)
+    opt.step()
+    saved = copy.deepcopy(opt.state_dict())
+    opt.step()
+    m = opt.state[p]["exp_avg"].clone()
+    bad = copy.deepcopy(saved)
+    bad["state"][1]["exp_avg"] = torch.zeros(31, device=DEV)
+    bad["param_groups"][0]["lr"] = 7.0
+    with pytest.raises(ValueError, match="exp_avg"):
+        opt.load_state_dict(bad)
+    bad = copy.deepcopy(saved)
+    bad["param_groups"][0]["amsgrad"] = True
+    with pytest.raises(ValueError, match="amsgrad"):
+        opt.load_state_dict(bad)
+    assert torch.equal(opt.state[p]["exp_avg"], m) and opt.param_groups[0]["lr"] == 1e-2
+    assert int(opt.state[q]["step"]) == 2
+    opt.step()
+    assert int(opt.state[p]["step"]) == 3
+
+
+def test_moments_of_16_bit_parameters_from_torch():
+    """torch keeps them in the parameter's type; here they are 32-bit"""
+    p = make([((50,), torch.bfloat16)], seed=23)[0]
+    q = p.detach().clone().requires_grad_()
+    q.grad = p.grad.clone()
+    a, b = torch.optim.AdamW([p], lr=1e-2), AdamW([q], lr=1e-2)
+    a.step()
+    b.load_state_dict(a.state_dict())
+    assert b.state[q]["exp_avg"].dtype == torch.float32
+    assert torch.equal(b.state[q]["exp_avg"], a.state[p]["exp_avg"].float())
+    with torch.no_grad():
+        q.copy_(p)
+    check_step(b, [q], 2, dict(lr=1e-2, b1=0.9, b2=0.999, eps=1e-8, wd=1e-2))
+
+
 def test_schedule_and_closure():
     p = make([((64,), torch.float32)], seed=12)[0]
     opt = AdamW([p], lr=0.1)
@@ -502,6 +539,31 @@ def test_replaced_state_is_seen():
     opt.param_groups[0].update(state_bits=32, lr=-1.0)
     with pytest.raises((ValueError, RuntimeError), match="lr"):
         opt.step()
+
+
+@pytest.mark.parametrize("python", [False, True])
+def test_refused_options_change_nothing(python, request):
+    if python:
+        request.getfixturevalue("python_path")
+    ps = make([((50,), torch.float32), ((60,), torch.float32)], seed=24)
+    opt = AdamW([dict(params=[ps[0]]), dict(params=[ps[1]])], lr=1e-2, max_norm=1.0)
+    opt.step()
+    was = [p.detach().clone() for p in ps]
+    for k, v in (("lr", -1.0), ("lr", float("nan")), ("betas", (0.9, 1.0)), ("eps", -1.0),
+                 ("weight_decay", -1.0)):
+        keep = opt.param_groups[1][k]
+        opt.param_groups[1][k] = v
+        with pytest.raises(ValueError):
+            opt.step()
+        opt.param_groups[1][k] = keep
+    assert all(torch.equal(p, q) for p, q in zip(ps, was))
+    assert [int(opt.state[p]["step"]) for p in ps] == [1, 1]
+    # another type in the same parameter: the state is 32-bit and stays
+    ps[0].data = ps[0].data.bfloat16()
+    ps[0].grad = torch.ones(50, device=DEV, dtype=torch.bfloat16)
+    opt.step()
+    assert int(opt.state[ps[0]]["step"]) == 2 and torch.isfinite(ps[0]).all()
+    assert (ps[0].float() - was[0]).abs().max() < 0.1
 
 
 def test_step_hooks_are_served():
