@@ -471,6 +471,11 @@ struct Handle {
 using FnGradNorm = decltype(&cqt_grad_norm);
 using FnAdamw = decltype(&cqt_adamw_step);
 
+// a kernel is about to change a tensor that autograd may have saved
+void written(const at::Tensor& t) {
+    if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // whether the elements fill one stretch of memory and element i of a's is
 // element i of b's (sizes are equal)
 bool same_order(const at::Tensor& a, const at::Tensor& b) {
@@ -506,6 +511,7 @@ struct AdamWPlan {
     std::vector<cqt_adamw_tensor> todo;
     std::vector<int64_t> ends;           // of each group in todo
     std::vector<at::Tensor> keep;
+    std::vector<const Slot*> stepped;    // the parameters behind todo
 
     static int32_t type_of(const at::Tensor& p) {
         return p.scalar_type() == at::kBFloat16 ? CQT_BF16
@@ -592,6 +598,7 @@ struct AdamWPlan {
         todo.clear();
         ends.clear();
         keep.clear();
+        stepped.clear();
         size_t k = 0;
         for (auto gr : param_groups) {
             Group& g = groups[k++];
@@ -639,6 +646,7 @@ struct AdamWPlan {
                     s.vs.defined() ? static_cast<uint8_t*>(s.vs.data_ptr()) : nullptr;
                 s.d.step = s.step.data_ptr<int64_t>();
                 todo.push_back(s.d);
+                stepped.push_back(&s);
             }
             ends.push_back((int64_t)todo.size());
         }
@@ -699,8 +707,15 @@ struct AdamWPlan {
                               "eps and weight_decay must not be negative");
             args.push_back(a);
         }
+        TORCH_CHECK_VALUE(!use_norm || args.empty() || args[0].max_norm > 0,
+                          "max_norm must be positive");
+        // autograd refuses a backward pass through values that it saved before
+        // the step, as behind any operation in place
+        for (const Slot* x : stepped)
+            for (const at::Tensor* t : {&x->p, &x->m, &x->v, &x->ms, &x->vs, &x->step, &x->master})
+                written(*t);
+        if (use_norm) written(*norm);
         if (use_norm) {
-            TORCH_CHECK_VALUE(args.empty() || args[0].max_norm > 0, "max_norm must be positive");
             check(norm_fn(todo.data(), (int)todo.size(), norm->data_ptr<float>(), ws.data_ptr(),
                           (size_t)ws.numel(), stream),
                   "cqt_grad_norm");

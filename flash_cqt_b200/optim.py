@@ -39,6 +39,12 @@ def _same_order(a, b):
     return all(x == y for x, y, n in zip(a.stride(), b.stride(), a.shape) if n != 1)
 
 
+def _written(tensors):
+    """autograd refuses a backward pass through what it saved of these before"""
+    torch.autograd.graph.increment_version(
+        [t for t in tensors if torch.is_tensor(t) and not t.is_inference()])
+
+
 def _reals(t):
     return t.numel() * (2 if t.is_complex() else 1)
 
@@ -352,7 +358,8 @@ class AdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def _lists(self):
         """the tensors of every group that have gradients, as the library takes
-        them (states are made and checked), and the copies behind them"""
+        them (states are made and checked), and (gradient or its copy, parameter,
+        state) of each"""
         lists, keep = [], []
         first = 0
         for g in self.param_groups:
@@ -365,7 +372,7 @@ class AdamW(torch.optim.Optimizer):
                 if not s:
                     s = self.state[p] = self._new_state(p, g)
                 grad = self._grad(p)
-                keep.append(grad)
+                keep.append((grad, p, s))
                 self._check_state(s, p, g)
                 at = lambda k: s[k].data_ptr() if k in s else None  # noqa: E731
                 todo.append(_native.CqtAdamwTensor(
@@ -379,6 +386,10 @@ class AdamW(torch.optim.Optimizer):
     def _python_step(self):
         with torch.cuda.device(self._dev):
             lists, keep = self._lists()
+            _written([t for _, p, s in keep for t in (p, *s.values())])
+            if self.max_norm is not None:
+                self._workspace(self._total)
+                _written([self.grad_norm])
             self._launch(lists)
 
     def _launch(self, lists):

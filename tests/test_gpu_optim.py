@@ -733,3 +733,32 @@ def test_train_step_with_the_transform():
     slope = (hi - lo) / (2 * h)
     # the loss is a mean of 131072 squares: a few steps of float32
     assert abs(slope - float(g.grad[k].real)) <= 8 * 2.0 ** -23 * max(hi, lo) / (2 * h)
+
+
+@pytest.mark.parametrize("python", [False, True])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_step_is_seen_by_autograd(bits, python, request):
+    """a backward pass through values that were saved before a step is refused,
+    as behind any operation in place"""
+    if python:
+        request.getfixturevalue("python_path")
+    ps = make([((50,), torch.float32), ((7, 3), torch.float32), ((4,), torch.float32)], seed=30)
+    opt = AdamW(ps, lr=1e-2, state_bits=bits, max_norm=1.0)
+    ps[2].grad = None
+    opt.step()
+    x = torch.ones((), device=DEV, requires_grad=True)
+    ys = [(p * p).sum() for p in ps] + [x * opt.grad_norm]
+    seen = [t._version for t in opt.state[ps[0]].values()]
+    opt.step()
+    for y in (ys[0], ys[1], ys[3]):
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    ys[2].backward()   # that one has not been stepped
+    assert torch.equal(ps[2].grad, 2 * ps[2].detach())
+    assert all(t._version > v for t, v in zip(opt.state[ps[0]].values(), seen))
+    # a refused step marks nothing
+    was = [p._version for p in ps]
+    opt.param_groups[0]["lr"] = -1.0
+    with pytest.raises(ValueError):
+        opt.step()
+    assert [p._version for p in ps] == was
