@@ -487,13 +487,38 @@ bool same_order(const at::Tensor& a, const at::Tensor& b) {
 // The parameters of an optimizer with the states that it holds for them.  It
 // remembers the Python objects that it was built from -- the lists of
 // parameters, the state dictionary, every parameter's own dictionary and what
-// is in them -- and refuses to step (the caller then builds another) when any of
-// them has been replaced.
+// is in them -- and refuses to step (the caller then checks them and builds
+// another) when any of them has been replaced, or when what a tensor of the state
+// holds is not of the type, device, size or order that the kernels take any
+// more (its storage can be exchanged without replacing the object).
 struct AdamWPlan {
     struct Slot {
         at::Tensor p;
         at::Tensor m, v, ms, vs, step, master;   // undefined: no state yet
         cqt_adamw_tensor d{};
+
+        // whether the state is what the kernels take for the parameter
+        bool fits(int bits) const {
+            const auto at_home = [&](const at::Tensor& t, at::ScalarType type) {
+                return t.defined() && t.scalar_type() == type && t.layout() == at::kStrided &&
+                       t.get_device() == p.get_device() && !t.is_conj() && !t.is_neg();
+            };
+            const auto like_p = [&](const at::Tensor& t, at::ScalarType type) {
+                return at_home(t, type) && t.sizes() == p.sizes() && same_order(t, p);
+            };
+            const auto flat = [&](const at::Tensor& t, at::ScalarType type, int64_t n) {
+                return at_home(t, type) && t.numel() == n && t.is_contiguous();
+            };
+            if (!at_home(step, at::kLong) || step.numel() != 1) return false;
+            if (master.defined() && !like_p(master, at::kFloat)) return false;
+            if (bits == 8) {
+                const int64_t blocks = (d.numel + 255) / 256;
+                return flat(m, at::kFloat8_e4m3fn, d.numel) && flat(v, at::kFloat8_e5m2, d.numel) &&
+                       flat(ms, at::kFloat8_e8m0fnu, blocks) && flat(vs, at::kFloat8_e8m0fnu, blocks);
+            }
+            const at::ScalarType type = p.is_complex() ? at::kComplexFloat : at::kFloat;
+            return like_p(m, type) && like_p(v, type);
+        }
     };
     struct Group {
         std::vector<Slot> slots;
@@ -627,9 +652,7 @@ struct AdamWPlan {
                 if (n != s.d.numel || type_of(p) != s.d.dtype || p.get_device() != device ||
                     !p.is_non_overlapping_and_dense() || p.is_conj() || p.is_neg())
                     return false;
-                if (g.bits == 32 && (s.m.sizes() != p.sizes() || !same_order(s.m, p) ||
-                                     s.v.sizes() != p.sizes() || !same_order(s.v, p)))
-                    return false;
+                if (!s.fits(g.bits)) return false;
                 at::Tensor use = grad;
                 if (grad.is_conj() || grad.is_neg() || !same_order(grad, p)) {
                     use = at::empty_like(p).copy_(grad);
@@ -651,6 +674,14 @@ struct AdamWPlan {
             ends.push_back((int64_t)todo.size());
         }
         return true;
+    }
+
+    // whether a step would take everything as it is
+    bool fits(pybind11::list param_groups, pybind11::dict state) {
+        at::NoGradGuard no_grad;
+        const bool yes = current(param_groups, state) && gather(param_groups);
+        keep.clear();
+        return yes;
     }
 
     // an option of a parameter group
@@ -709,6 +740,9 @@ struct AdamWPlan {
         }
         TORCH_CHECK_VALUE(!use_norm || args.empty() || args[0].max_norm > 0,
                           "max_norm must be positive");
+        TORCH_CHECK_VALUE(!use_norm || (norm->get_device() == device && norm->numel() == 1 &&
+                                        norm->scalar_type() == at::kFloat),
+                          "grad_norm must hold one float32 number on cuda:", (int)device);
         // autograd refuses a backward pass through values that it saved before
         // the step, as behind any operation in place
         for (const Slot* x : stepped)
@@ -907,6 +941,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         .def("last_heap", &Handle::last_heap);
     pybind11::class_<AdamWPlan>(m, "AdamWPlan")
         .def(pybind11::init<int, uintptr_t, uintptr_t, uintptr_t, pybind11::list, pybind11::dict>())
+        .def("fits", &AdamWPlan::fits)
         .def("step", &AdamWPlan::step);
     pybind11::class_<CacheHandle>(m, "CacheHandle")
         .def(pybind11::init<uintptr_t, uintptr_t, uintptr_t, at::Tensor, at::Tensor, at::Tensor,

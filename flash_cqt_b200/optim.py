@@ -143,6 +143,19 @@ class AdamW(torch.optim.Optimizer):
         if g["state_bits"] not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32, got {g['state_bits']}")
 
+    def _check_param(self, p):
+        if p.dtype not in _TYPES:
+            raise TypeError("parameters must be float32, bfloat16, float16 or complex64, "
+                            f"got {p.dtype}")
+        if p.is_conj() or p.is_neg() or not _dense(p):
+            raise ValueError("parameters must be dense in memory (no gaps, no elements "
+                             "that share a place, no lazy conjugate)")
+        if p.device.type != "cuda":
+            raise RuntimeError(f"the optimizer step runs on CUDA devices only, got {p.device} "
+                               "(there is no CPU fallback)")
+        if self._dev is not None and p.device != self._dev:
+            raise ValueError(f"parameters must be on one device: {p.device}, {self._dev}")
+
     def add_param_group(self, group):
         group = dict(group)
         params = group["params"]
@@ -156,17 +169,7 @@ class AdamW(torch.optim.Optimizer):
         for p in tensors:
             if not torch.is_tensor(p):
                 raise TypeError(f"parameters must be tensors, got {type(p).__name__}")
-            if p.dtype not in _TYPES:
-                raise TypeError("parameters must be float32, bfloat16, float16 or complex64, "
-                                f"got {p.dtype}")
-            if p.is_conj() or p.is_neg() or not _dense(p):
-                raise ValueError("parameters must be dense in memory (no gaps, no elements "
-                                 "that share a place, no lazy conjugate)")
-            if p.device.type != "cuda":
-                raise RuntimeError(f"the optimizer step runs on CUDA devices only, got {p.device} "
-                                   "(there is no CPU fallback)")
-            if self._dev is not None and p.device != self._dev:
-                raise ValueError(f"parameters must be on one device: {p.device}, {self._dev}")
+            self._check_param(p)
             self._dev = p.device
             spans += self._span(p)
         spans.sort()
@@ -218,7 +221,8 @@ class AdamW(torch.optim.Optimizer):
         want["step"] = torch.int64
         for k, dt in want.items():
             t = s.get(k)
-            if not torch.is_tensor(t) or t.dtype != dt or t.device != p.device:
+            if not torch.is_tensor(t) or t.dtype != dt or t.device != p.device \
+                    or t.layout != torch.strided or t.is_conj() or t.is_neg():
                 raise ValueError(f"state {k!r} must be a {dt} tensor on {p.device}")
             if k == "step":
                 fits = t.numel() == 1
@@ -368,6 +372,7 @@ class AdamW(torch.optim.Optimizer):
             for k, p in enumerate(g["params"]):
                 if p.grad is None or not p.numel():
                     continue
+                self._check_param(p)   # its storage may have been exchanged
                 s = self.state.get(p)
                 if not s:
                     s = self.state[p] = self._new_state(p, g)
@@ -386,10 +391,13 @@ class AdamW(torch.optim.Optimizer):
     def _python_step(self):
         with torch.cuda.device(self._dev):
             lists, keep = self._lists()
-            _written([t for _, p, s in keep for t in (p, *s.values())])
             if self.max_norm is not None:
                 self._workspace(self._total)
-                _written([self.grad_norm])
+                n = self.grad_norm
+                if n.device != self._dev or n.numel() != 1 or n.dtype != torch.float32:
+                    raise ValueError(f"grad_norm must hold one float32 number on {self._dev}")
+                _written([n])
+            _written([t for _, p, s in keep for t in (p, *s.values())])
             self._launch(lists)
 
     def _launch(self, lists):

@@ -762,3 +762,43 @@ def test_step_is_seen_by_autograd(bits, python, request):
     with pytest.raises(ValueError):
         opt.step()
     assert [p._version for p in ps] == was
+
+
+@pytest.mark.parametrize("python", [False, True])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_exchanged_storage_is_refused(bits, python, request):
+    """a state whose storage was moved away or replaced behind the same object
+    is refused before anything is launched"""
+    if python:
+        request.getfixturevalue("python_path")
+    ps = make([((4, 130), torch.bfloat16), ((300,), torch.bfloat16)], seed=31)
+    opt = AdamW(ps, lr=1e-2, state_bits=bits, master=True, max_norm=1.0)
+    opt.step()
+    was = [p.detach().clone() for p in ps]
+    for k in list(opt.state[ps[1]]):
+        t = opt.state[ps[1]][k]
+        for other in (t.data.cpu(), t.data.double() if k != "step" else t.data.int()):
+            keep = t.data
+            t.data = other
+            with pytest.raises(ValueError, match=k):
+                opt.step()
+            t.data = keep
+    p = ps[1]
+    keep, grad = p.data, p.grad
+    for other in (keep.cpu(), torch.zeros(300, 2, dtype=torch.bfloat16, device=DEV)[:, 0]):
+        p.grad = None
+        p.data = other
+        p.grad = torch.ones_like(p)
+        with pytest.raises((RuntimeError, ValueError), match="CUDA devices only|dense"):
+            opt.step()
+    p.grad = None
+    p.data = keep
+    p.grad = grad
+    norm = opt.grad_norm
+    opt.grad_norm = norm.cpu()
+    with pytest.raises(ValueError, match="grad_norm"):
+        opt.step()
+    opt.grad_norm = norm
+    assert all(torch.equal(p.detach(), q) for p, q in zip(ps, was))
+    opt.step()
+    assert [int(opt.state[p]["step"]) for p in ps] == [2, 2]

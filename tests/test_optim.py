@@ -126,3 +126,75 @@ def test_rounding_is_unbiased():
     v[::po.BLOCK] = 57344.0
     r = po.round_v(v, po.scales(v, 57344.0), po.noise(1, 1, 0, n))[v == 3.3]
     assert abs(r.mean() - 3.3) < 6 * 0.25 / np.sqrt(r.size)
+
+
+def state_of(p, bits, master=False):
+    """a state as the kernels take it, on the parameter's device"""
+    n = p.numel() * (2 if p.is_complex() else 1)
+    s = dict(step=torch.zeros((), dtype=torch.int64, device=p.device))
+    if bits == 8:
+        z = lambda n, dt: torch.ones(n, dtype=torch.uint8, device=p.device).view(dt)  # noqa: E731
+        s.update(exp_avg=z(n, torch.float8_e4m3fn), exp_avg_sq=z(n, torch.float8_e5m2),
+                 exp_avg_scale=z(-(-n // 256), torch.float8_e8m0fnu),
+                 exp_avg_sq_scale=z(-(-n // 256), torch.float8_e8m0fnu))
+    else:
+        dt = torch.complex64 if p.is_complex() else torch.float32
+        s.update(exp_avg=torch.zeros_like(p, dtype=dt, requires_grad=False),
+                 exp_avg_sq=torch.zeros_like(p, dtype=dt, requires_grad=False))
+    if master:
+        s["master"] = p.detach().float()
+    return s
+
+
+def exchanges(bits, master):
+    """(entry, what is put in its place): another type, size or order"""
+    every = ["exp_avg", "exp_avg_sq", "step"] + (["master"] if master else []) \
+        + (["exp_avg_scale", "exp_avg_sq_scale"] if bits == 8 else [])
+    out = []
+    for k in every:
+        out.append((k, lambda x: x.float().double() if x.dtype != torch.int64 else x.int()))
+        out.append((k, lambda x: torch.cat([x.reshape(-1).view(torch.uint8)] * 2).view(x.dtype)))
+        if k == "master" or (bits == 32 and k != "step"):
+            out.append((k, lambda x: x.t().contiguous().t()))
+            out.append((k, lambda x: x.bfloat16()))
+            out.append((k, lambda x: x.t()))
+        elif k != "step":
+            out.append((k, lambda x: x[:-1]))
+            out.append((k, lambda x: x.view(torch.uint8)))
+            out.append((k, lambda x: torch.cat([x.view(torch.uint8)] * 2).view(x.dtype)[::2]))
+    return out
+
+
+@pytest.mark.parametrize("bits, master", [(32, False), (32, True), (8, False), (8, True)])
+def test_exchanged_states_are_refused(bits, master):
+    """every tensor of a state is looked at again before a step: its storage
+    can be exchanged behind the same object"""
+    mod = _native.torch_ops()
+    dt = torch.bfloat16 if master else torch.float32
+    p, q = (torch.zeros(5, 120, dtype=dt, requires_grad=True) for _ in range(2))
+    for x in (p, q):
+        x.grad = torch.ones_like(x)
+    group = dict(params=[p, q], state_bits=bits, master=master)
+    state = {x: state_of(x, bits, master) for x in (p, q)}
+    plan = mod.AdamWPlan(-1, 0, 0, 0, [group], state)
+    assert plan.fits([group], state)
+    for k, change in exchanges(bits, master):
+        was = state[q][k].data
+        state[q][k].data = change(was)
+        assert not plan.fits([group], state), k
+        with pytest.raises(ValueError, match=k):
+            AdamW._check_state(state[q], q, group)
+        state[q][k].data = was
+        assert plan.fits([group], state)
+    # the parameter's own
+    was = p.data
+    for other in (was.double(), was[:, :7]):
+        p.data = other
+        p.grad = None
+        assert plan.fits([group], state)   # nothing is done with it
+        p.grad = torch.ones_like(p)
+        assert not plan.fits([group], state)
+    p.data, p.grad = was, None
+    p.grad = torch.ones_like(p)
+    assert plan.fits([group], state)
+    AdamW._check_state(state[p], p, group)
