@@ -495,7 +495,17 @@ struct AdamWPlan {
     struct Slot {
         at::Tensor p;
         at::Tensor m, v, ms, vs, step, master;   // undefined: no state yet
+        std::vector<int64_t> sizes, strides;     // of the parameter when it was checked
         cqt_adamw_tensor d{};
+
+        // whether the parameter has the memory order that its state was checked
+        // for: the codes of 8-bit moments are flat and do not show theirs
+        bool in_order() const {
+            if (p.sizes() != at::IntArrayRef(sizes)) return false;
+            for (size_t k = 0; k < sizes.size(); ++k)
+                if (sizes[k] != 1 && p.stride((int64_t)k) != strides[k]) return false;
+            return true;
+        }
 
         // whether the state is what the kernels take for the parameter
         bool fits(int bits) const {
@@ -575,6 +585,8 @@ struct AdamWPlan {
                 out.slots.emplace_back();
                 Slot& s = out.slots.back();
                 s.p = p.cast<at::Tensor>();
+                s.sizes = s.p.sizes().vec();
+                s.strides = s.p.strides().vec();
                 s.d.ordinal = ordinal++;
                 s.d.numel = s.p.numel() * (s.p.is_complex() ? 2 : 1);
                 s.d.dtype = type_of(s.p);
@@ -652,7 +664,7 @@ struct AdamWPlan {
                 if (n != s.d.numel || type_of(p) != s.d.dtype || p.get_device() != device ||
                     !p.is_non_overlapping_and_dense() || p.is_conj() || p.is_neg())
                     return false;
-                if (!s.fits(g.bits)) return false;
+                if (!s.in_order() || !s.fits(g.bits)) return false;
                 at::Tensor use = grad;
                 if (grad.is_conj() || grad.is_neg() || !same_order(grad, p)) {
                     use = at::empty_like(p).copy_(grad);

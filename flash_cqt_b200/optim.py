@@ -24,19 +24,65 @@ _TYPES = {torch.float32: _native.CQT_F32, torch.bfloat16: _native.CQT_BF16,
           torch.float16: _native.CQT_F16, torch.complex64: _native.CQT_F32}
 
 
-def _dense(t):
-    """whether the elements fill one stretch of memory, in any order of dims"""
+def _fills(shape, strides):
+    """whether elements at these strides fill one stretch of memory"""
     want = 1
-    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+    for stride, size in sorted((s, n) for s, n in zip(strides, shape) if n != 1):
         if stride != want:
             return False
         want *= size
     return True
 
 
+def _dense(t):
+    """whether the elements fill one stretch of memory, in any order of dims"""
+    return _fills(t.shape, t.stride())
+
+
 def _same_order(a, b):
     """whether element i of a's memory is element i of b's (both dense)"""
     return all(x == y for x, y, n in zip(a.stride(), b.stride(), a.shape) if n != 1)
+
+
+def _order(p):
+    """the memory order of a dense tensor: its sizes over its strides"""
+    return torch.tensor([list(p.shape), list(p.stride())], dtype=torch.int64)
+
+
+def _ordered_like(order, p):
+    shape, strides = order.tolist()
+    return shape == list(p.shape) and all(
+        a == b for a, b, n in zip(strides, p.stride(), shape) if n != 1)
+
+
+def _values8(codes, scales):
+    """8-bit moments as float32"""
+    return codes.float() * scales.float().repeat_interleave(BLOCK)[:codes.numel()]
+
+
+def _codes8(x, dtype):
+    """(codes, scales) of flat float32 values, rounded to nearest"""
+    b = torch.nn.functional.pad(x, (0, -x.numel() % BLOCK)).view(-1, BLOCK)
+    top = torch.where(b.isfinite(), b.abs(), 0.0).amax(1)
+    # the least 2^k with top <= 1.75 * 2^8 (e4m3) or 1.75 * 2^15 (e5m2) of it
+    k = ((top.view(torch.int32) + 0x1fffff >> 23) - (8 if dtype == torch.float8_e4m3fn else 15)
+         ).clamp_min(1)
+    y = b * (254 - k << 23).view(torch.float32)[:, None]
+    if dtype == torch.float8_e5m2:   # a denominator must not vanish
+        y = torch.where(b > 0, y.clamp_min(2.0 ** -14), y)
+    return (y.view(-1)[:x.numel()].to(dtype),
+            k.to(torch.uint8).view(torch.float8_e8m0fnu))
+
+
+def _relaid(x, order, p):
+    """flat values of the elements of ``p`` in another memory order, in p's own"""
+    def as_p(x, shape, strides):
+        if p.is_complex():   # (re, im) of an element lie together
+            shape, strides = [*shape, 2], [*(2 * s for s in strides), 1]
+        return x.as_strided(shape, strides)
+    out = torch.empty_like(x)
+    as_p(out, p.shape, p.stride()).copy_(as_p(x, *order.tolist()))
+    return out
 
 
 def _written(tensors):
@@ -80,9 +126,13 @@ class AdamW(torch.optim.Optimizer):
     captured.
 
     ``state_bits=8`` holds the moments in 8 bits: ``exp_avg`` as float8_e4m3fn
-    and ``exp_avg_sq`` as float8_e5m2 values in the parameter's memory order,
-    256 of which share a power-of-two scale (``exp_avg_scale``,
-    ``exp_avg_sq_scale``, float8_e8m0fnu).  They are rounded stochastically by a
+    and ``exp_avg_sq`` as float8_e5m2 values in the parameter's memory order
+    (``order``: its sizes and strides, int64 [2, dim] on the host; a state without
+    it is of a contiguous parameter), 256 of which share a power-of-two scale
+    (``exp_avg_scale``, ``exp_avg_sq_scale``, float8_e8m0fnu).  A step refuses a
+    parameter whose order has changed; a state that was saved in another order is
+    laid out anew when it is loaded, which rounds only what is small beside its
+    new neighbours.  They are rounded stochastically by a
     hash of (``seed``, t, the parameter's number, element): the same run gives
     the same bits.  ``master=True`` keeps a 32-bit copy of a 16-bit parameter,
     which is then its rounding; without it a 16-bit parameter loses updates
@@ -198,6 +248,7 @@ class AdamW(torch.optim.Optimizer):
             for k in ("exp_avg_scale", "exp_avg_sq_scale"):
                 s[k] = zeros(-(-n // BLOCK), torch.float8_e8m0fnu)
                 s[k].view(torch.uint8).fill_(1)
+            s["order"] = _order(p)
         else:
             dt = torch.complex64 if p.is_complex() else torch.float32
             s["exp_avg"] = torch.zeros_like(p, dtype=dt, requires_grad=False)
@@ -233,6 +284,16 @@ class AdamW(torch.optim.Optimizer):
                 fits = t.shape == p.shape and _dense(t) and _same_order(t, p)
             if not fits:
                 raise ValueError(f"state {k!r} does not fit its parameter {tuple(p.shape)}")
+        if eight:
+            o = s.get("order")
+            if o is None:
+                if not p.is_contiguous():
+                    raise ValueError("state 'order' is missing: 8-bit moments without it are "
+                                     "those of a contiguous parameter")
+            elif not torch.is_tensor(o) or o.dtype != torch.int64 or o.shape != (2, p.dim()) \
+                    or not _ordered_like(o, p):
+                raise ValueError("state 'order': the 8-bit moments lie in another memory order "
+                                 f"than their parameter {tuple(p.shape)}, {p.stride()}")
 
     @torch.no_grad()
     def init_state(self):
@@ -281,19 +342,34 @@ class AdamW(torch.optim.Optimizer):
     def _loaded(self, saved, p, g):
         """a parameter's saved state as new tensors, laid out for the kernels"""
         s = {}
+        eight = g["state_bits"] == 8
         for k, v in saved.items():
+            if k == "order":
+                continue
             if k == "step":
                 s[k] = torch.as_tensor(v).detach().to(p.device, torch.int64).reshape(()).clone()
             elif torch.is_tensor(v):
                 v = v.detach().to(p.device, copy=True)
-                if g["state_bits"] == 32 and v.dtype in (torch.bfloat16, torch.float16):
+                if not eight and v.dtype in (torch.bfloat16, torch.float16):
                     v = v.float()   # moments that were kept in the parameter's type
                 if v.shape == p.shape and not _same_order(v, p):
                     v = torch.empty_like(p, dtype=v.dtype, requires_grad=False).copy_(v)
                 s[k] = v
         if g["master"] and "master" not in s and p.dtype in (torch.bfloat16, torch.float16):
             s["master"] = p.detach().float()
+        order = saved.get("order")
+        if eight and order is not None:
+            s["order"] = _order(p)
         self._check_state(s, p, g)
+        if eight and order is not None:
+            order = torch.as_tensor(order).cpu()
+            if order.shape != (2, p.dim()) or order[0].tolist() != list(p.shape) \
+                    or not _fills(*order.tolist()):
+                raise ValueError(f"state 'order' does not fit its parameter {tuple(p.shape)}")
+            if not _ordered_like(order, p):
+                for k in ("exp_avg", "exp_avg_sq"):
+                    s[k], s[k + "_scale"] = _codes8(
+                        _relaid(_values8(s[k], s[k + "_scale"]), order, p), s[k].dtype)
         return s
 
     # -------------------------------------------------------------------- step
@@ -379,6 +455,8 @@ class AdamW(torch.optim.Optimizer):
                 grad = self._grad(p)
                 keep.append((grad, p, s))
                 self._check_state(s, p, g)
+                if g["state_bits"] == 8:
+                    s.setdefault("order", _order(p))
                 at = lambda k: s[k].data_ptr() if k in s else None  # noqa: E731
                 todo.append(_native.CqtAdamwTensor(
                     p.data_ptr(), grad.data_ptr(), at("master") if g["master"] else None,

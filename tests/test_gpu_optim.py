@@ -748,14 +748,15 @@ def test_step_is_seen_by_autograd(bits, python, request):
     opt.step()
     x = torch.ones((), device=DEV, requires_grad=True)
     ys = [(p * p).sum() for p in ps] + [x * opt.grad_norm]
-    seen = [t._version for t in opt.state[ps[0]].values()]
+    state = [t for k, t in opt.state[ps[0]].items() if k != "order"]   # (never written)
+    seen = [t._version for t in state]
     opt.step()
     for y in (ys[0], ys[1], ys[3]):
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             y.backward()
     ys[2].backward()   # that one has not been stepped
     assert torch.equal(ps[2].grad, 2 * ps[2].detach())
-    assert all(t._version > v for t, v in zip(opt.state[ps[0]].values(), seen))
+    assert all(t._version > v for t, v in zip(state, seen))
     # a refused step marks nothing
     was = [p._version for p in ps]
     opt.param_groups[0]["lr"] = -1.0
@@ -775,7 +776,7 @@ def test_exchanged_storage_is_refused(bits, python, request):
     opt = AdamW(ps, lr=1e-2, state_bits=bits, master=True, max_norm=1.0)
     opt.step()
     was = [p.detach().clone() for p in ps]
-    for k in list(opt.state[ps[1]]):
+    for k in [k for k in opt.state[ps[1]] if k != "order"]:   # (no kernel takes that)
         t = opt.state[ps[1]][k]
         for other in (t.data.cpu(), t.data.double() if k != "step" else t.data.int()):
             keep = t.data
@@ -802,3 +803,60 @@ def test_exchanged_storage_is_refused(bits, python, request):
     assert all(torch.equal(p.detach(), q) for p, q in zip(ps, was))
     opt.step()
     assert [int(opt.state[p]["step"]) for p in ps] == [2, 2]
+
+
+@pytest.mark.parametrize("python", [False, True])
+@pytest.mark.parametrize("bits, master", [(32, False), (32, True), (8, False), (8, True)])
+def test_changed_order_is_refused(bits, master, python, request):
+    """a parameter that is moved to another memory order behind the same object"""
+    if python:
+        request.getfixturevalue("python_path")
+    p = make([((4, 6, 3, 5), torch.bfloat16)], seed=32)[0]
+    opt = AdamW([p], lr=1e-2, state_bits=bits, master=master)
+    opt.step()
+    was, m = p.detach().clone(), opt.state[p]["exp_avg"].clone()
+    p.data = p.data.to(memory_format=torch.channels_last)
+    with pytest.raises(ValueError, match="order" if bits == 8 and not master else "state"):
+        opt.step()
+    assert torch.equal(p.detach(), was) and int(opt.state[p]["step"]) == 1
+    assert torch.equal(opt.state[p]["exp_avg"].float(), m.float())
+    p.data = p.data.contiguous()
+    check_step(opt, [p], 2, dict(lr=1e-2, b1=0.9, b2=0.999, eps=1e-8, wd=1e-2), bits, master)
+
+
+@pytest.mark.parametrize("dtype, master", [(torch.float32, False), (torch.complex64, False),
+                                           (torch.bfloat16, True)])
+def test_state_of_another_order(dtype, master):
+    """8-bit moments saved from a contiguous parameter go on with one in another
+    order, and the way back"""
+    kw = dict(lr=1e-2, b1=0.9, b2=0.999, eps=1e-8, wd=1e-2)
+    p = make([((4, 6, 3, 50), dtype)], seed=33)[0]
+    other = p.detach().permute(0, 2, 3, 1).contiguous().permute(0, 3, 1, 2)
+    q = other.requires_grad_()
+    a = AdamW([p], lr=1e-2, state_bits=8, master=master)
+    a.step()
+    b = AdamW([q], lr=1e-2, state_bits=8, master=master)
+    b.load_state_dict(a.state_dict())
+    with torch.no_grad():
+        q.copy_(p)
+    q.grad = p.grad.clone()   # in the other order: copied for the step
+
+    def moments(opt, x):
+        """element by element, in the order of the indices"""
+        shape = (*x.shape, 2) if x.is_complex() else tuple(x.shape)
+        strides = (*(2 * t for t in x.stride()), 1) if x.is_complex() else x.stride()
+        return [torch.from_numpy(values8(opt.state[x], k)).as_strided(shape, strides)
+                for k in ("exp_avg", "exp_avg_sq")]
+    for x, y, small in zip(moments(a, p), moments(b, q), (2.0 ** -6, 2.0 ** -14)):
+        # what is small beside its new neighbours rounds: a scale is at most 2^-8
+        # (2^-15) of the largest value over 0.875
+        top = float(x.abs().max())
+        assert ((x - y).abs() <= (top / 0.875 * 2.0 ** (-8 if small > 1e-3 else -15)) * small).all()
+        assert ((x - y).abs() == 0).double().mean() > 0.5
+    q.grad = torch.empty_like(q).copy_(p.grad)
+    check_step(b, [q], 2, kw, 8, master)
+    c = AdamW([p], lr=1e-2, state_bits=8, master=master)
+    c.load_state_dict(b.state_dict())
+    with torch.no_grad():
+        p.copy_(q)
+    check_step(c, [p], 3, kw, 8, master)

@@ -188,7 +188,7 @@ def test_exchanged_states_are_refused(bits, master):
         assert plan.fits([group], state)
     # the parameter's own
     was = p.data
-    for other in (was.double(), was[:, :7]):
+    for other in (was.double(), was[:, :7], was.t().contiguous().t(), was.t()):
         p.data = other
         p.grad = None
         assert plan.fits([group], state)   # nothing is done with it
@@ -198,3 +198,107 @@ def test_exchanged_states_are_refused(bits, master):
     p.grad = torch.ones_like(p)
     assert plan.fits([group], state)
     AdamW._check_state(state[p], p, group)
+
+
+@pytest.fixture
+def on_host(monkeypatch):
+    """optimizers over host tensors: everything but the step itself"""
+    monkeypatch.setattr(AdamW, "_check_param", lambda self, p: None)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+
+
+def values(s, p):
+    """an 8-bit state's moments as float64, element by element of the parameter"""
+    out = []
+    for k in ("exp_avg", "exp_avg_sq"):
+        x = s[k].double() * s[k + "_scale"].double().repeat_interleave(256)[:s[k].numel()]
+        shape, strides = list(p.shape), list(p.stride())
+        if p.is_complex():
+            shape, strides = [*shape, 2], [*(2 * t for t in strides), 1]
+        out.append(x.as_strided(shape, strides))
+    return out
+
+
+def random_codes(s, seed):
+    """normal values (and zero) of both formats, scales of a few binades"""
+    g = torch.Generator().manual_seed(seed)
+    n = s["exp_avg"].numel()
+    r = lambda lo, hi, m=n: torch.randint(lo, hi, (m,), generator=g, dtype=torch.uint8)  # noqa: E731
+    s["exp_avg"].view(torch.uint8).copy_(r(64, 127) | r(0, 2) << 7)     # 2 to 448
+    s["exp_avg"].view(torch.uint8)[::17] = 0
+    s["exp_avg_sq"].view(torch.uint8).copy_(r(60, 124))                 # 1 to 57344
+    for k in ("exp_avg_scale", "exp_avg_sq_scale"):
+        s[k].view(torch.uint8).copy_(r(100, 106, s[k].numel()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.complex64])
+def test_codes_are_laid_out_anew(on_host, dtype):
+    """8-bit moments that were saved in another memory order keep their elements"""
+    a = torch.zeros(3, 5, 7, 4, dtype=dtype, requires_grad=True)
+    b = torch.zeros(3, 5, 7, 4, dtype=dtype).permute(0, 2, 3, 1).contiguous().permute(0, 3, 1, 2)
+    b.requires_grad_()
+    assert a.shape == b.shape and a.stride() != b.stride()
+    for p, q in ((a, b), (b, a), (a, a), (b, b)):
+        one, two = AdamW([p], state_bits=8), AdamW([q], state_bits=8)
+        one.init_state()
+        random_codes(one.state[p], seed=5)
+        two.load_state_dict(one.state_dict())
+        for x, y in zip(values(one.state[p], p), values(two.state[q], q)):
+            assert torch.equal(x, y)   # no value is 2^-6 (m) or 2^-14 (v) of a neighbour's scale
+        AdamW._check_state(two.state[q], q, two.param_groups[0])
+        assert two.state[q]["order"].tolist() == [list(q.shape), list(q.stride())]
+
+
+def test_codes_small_beside_new_neighbours(on_host):
+    """what falls under its new block's scale: m goes to the nearest value, v never
+    to zero; infinite and undefined values stay what they are"""
+    p = torch.zeros(256, 2, requires_grad=True)
+    q = torch.zeros(2, 256).t().requires_grad_()
+    one, two = AdamW([p], state_bits=8), AdamW([q], state_bits=8)
+    one.init_state()
+    s = one.state[p]
+    s["exp_avg"].view(torch.uint8).fill_(0x38)       # 1
+    s["exp_avg_sq"].view(torch.uint8).fill_(0x3c)    # 1
+    for k in ("exp_avg_scale", "exp_avg_sq_scale"):
+        s[k].view(torch.uint8)[:] = torch.tensor([127, 87], dtype=torch.uint8)   # 1 and 2^-40
+    s["exp_avg"].view(torch.uint8)[3] = 0x7f         # NaN
+    s["exp_avg_sq"].view(torch.uint8)[5] = 0x7c      # inf
+    s["exp_avg_sq"].view(torch.uint8)[300] = 0
+    two.load_state_dict(one.state_dict())
+    (m0, v0), (m1, v1) = values(s, p), values(two.state[q], q)
+    big = torch.arange(256) < 128
+    assert torch.equal(m1[~big], torch.zeros(128, 2).double())
+    assert torch.equal(torch.nan_to_num(m1[big], 9.0), torch.nan_to_num(m0[big], 9.0))
+    assert m1.isnan().sum() == 1 and v1.isinf().sum() == 1
+    assert torch.equal(v1[big], v0[big])
+    # the columns' largest value is 1: scales 2^-15, their smallest normal value 2^-29
+    assert v1[150, 0] == 0 and (v1[~big] == 2.0 ** -29).sum() == 255
+
+
+def test_order_refusals(on_host):
+    p = torch.zeros(6, 40, requires_grad=True)
+    q = torch.zeros(40, 6).t().requires_grad_()
+    one, two = AdamW([p], state_bits=8), AdamW([q], state_bits=8)
+    one.init_state()
+    saved = one.state_dict()
+
+    def without(key, value=None):
+        s = {k: v for k, v in saved["state"][0].items() if k != key}
+        return dict(saved, state={0: s if value is None else dict(s, **{key: value})})
+    one.load_state_dict(without("order"))            # a contiguous parameter: fine
+    AdamW._check_state(one.state[p], p, one.param_groups[0])
+    with pytest.raises(ValueError, match="order"):
+        two.load_state_dict(without("order"))
+    for bad in (torch.tensor([[6, 40], [40, 2]]), torch.tensor([[40, 6], [6, 1]]),
+                torch.tensor([[6, 40, 1], [40, 1, 1]]), torch.tensor([[6, 40], [1 << 40, 1]])):
+        with pytest.raises(ValueError, match="order"):
+            one.load_state_dict(without("order", bad))
+    # a parameter that was moved to another order after its state was made
+    group = one.param_groups[0]
+    plan = _native.torch_ops().AdamWPlan(-1, 0, 0, 0, one.param_groups, one.state)
+    p.grad = torch.ones(6, 40)
+    assert plan.fits(one.param_groups, one.state)
+    p.data = p.data.t().contiguous().t()
+    assert not plan.fits(one.param_groups, one.state)
+    with pytest.raises(ValueError, match="order"):
+        AdamW._check_state(one.state[p], p, group)
