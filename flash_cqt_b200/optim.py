@@ -318,9 +318,9 @@ class AdamW(torch.optim.Optimizer):
             # the base class would cast the state to the parameters' types: it
             # only takes the groups, the state is laid out here
             super().load_state_dict(dict(state_dict, state={}))
-            for g in self.param_groups:
-                for k, v in self.defaults.items():
-                    g.setdefault(k, v)
+            for g, old in zip(self.param_groups, was):
+                for k, v in self.defaults.items():   # what is not said there stays
+                    g.setdefault(k, old.get(k, v))
             new = {p: self._loaded(state_dict["state"][i], p, g)
                    for old, g in zip(groups, self.param_groups)
                    for i, p in zip(old["params"], g["params"]) if state_dict["state"].get(i)}

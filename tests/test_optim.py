@@ -302,3 +302,32 @@ def test_order_refusals(on_host):
     assert not plan.fits(one.param_groups, one.state)
     with pytest.raises(ValueError, match="order"):
         AdamW._check_state(one.state[p], p, group)
+
+
+def torch_state(*shapes, dtype=torch.float32, **kw):
+    """the state of torch's own AdamW after a step"""
+    ps = [torch.ones(*s, dtype=dtype, requires_grad=True) for s in shapes]
+    opt = torch.optim.AdamW(ps, **kw)
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    return opt.state_dict()
+
+
+def test_loaded_dictionary_leaves_a_groups_own_options(on_host):
+    """what a dictionary does not name stays as the group has it"""
+    p, q = leaf(5, dtype=torch.bfloat16), leaf(6)
+    groups = [dict(params=[p], master=True, eps=1e-6), dict(params=[q], state_bits=8)]
+    opt = AdamW(groups, lr=1e-2)
+    saved = torch_state((5,), dtype=torch.bfloat16, lr=3e-4)
+    saved["param_groups"].append(dict(params=[1], lr=7e-4))
+    opt.load_state_dict(saved)
+    a, b = opt.param_groups
+    assert a["master"] is True and a["state_bits"] == 32 and a["lr"] == 3e-4 and a["eps"] == 1e-8
+    assert opt.state[p]["master"].dtype == torch.float32
+    assert b["state_bits"] == 8 and b["master"] is False and b["lr"] == 7e-4 and b["eps"] == 1e-8
+    # 32-bit moments for a group that keeps 8 bits: refused, not turned over
+    saved["state"][1] = torch_state((6,))["state"][0]
+    with pytest.raises(ValueError, match="exp_avg"):
+        opt.load_state_dict(saved)
+    assert opt.param_groups[1]["state_bits"] == 8
