@@ -146,8 +146,8 @@ class AdamW(torch.optim.Optimizer):
     Steps of one optimizer must be ordered on one stream at a time.  State is
     made at a parameter's first step; before a step is captured it has to be
     there (``init_state()``, or a step).  ``load_state_dict`` (which also takes the
-    state of ``torch.optim.AdamW``) writes into the state that is there, so a
-    captured step goes on from what was loaded.
+    state of ``torch.optim.AdamW``) writes into the state, and into a rate on the
+    device, that are there, so a captured step goes on from what was loaded.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *,
@@ -321,6 +321,7 @@ class AdamW(torch.optim.Optimizer):
             for g, old in zip(self.param_groups, was):
                 for k, v in self.defaults.items():   # what is not said there stays
                     g.setdefault(k, old.get(k, v))
+            rates = self._keep_rates(was)
             new = {p: self._loaded(state_dict["state"][i], p, g)
                    for old, g in zip(groups, self.param_groups)
                    for i, p in zip(old["params"], g["params"]) if state_dict["state"].get(i)}
@@ -329,6 +330,8 @@ class AdamW(torch.optim.Optimizer):
             self.state.clear()
             self.state.update(before)
             raise
+        for at, rate in rates.items():
+            at.fill_(rate)
         for p, s in new.items():
             # into the tensors that are there: a captured step goes on with them
             for k, v in s.items():
@@ -338,6 +341,22 @@ class AdamW(torch.optim.Optimizer):
                     s[k] = at.copy_(v)
         self.state.clear()
         self.state.update(new)
+
+    def _keep_rates(self, was):
+        """puts rates that are device tensors back into groups that were loaded (a
+        captured step reads them): {tensor: the number that was loaded}"""
+        rates = {}
+        for g, old in zip(self.param_groups, was):
+            at, lr = old["lr"], g["lr"]
+            if not torch.is_tensor(at) or at.device != self._dev:
+                continue
+            if torch.is_tensor(lr) and lr.numel() != 1:
+                raise ValueError(f"a tensor lr must hold one number, got {tuple(lr.shape)}")
+            if rates.setdefault(at, float(lr)) != float(lr):
+                raise ValueError("parameter groups that share one lr tensor cannot take "
+                                 f"different rates: {rates[at]}, {float(lr)}")
+            g["lr"] = at
+        return rates
 
     def _loaded(self, saved, p, g):
         """a parameter's saved state as new tensors, laid out for the kernels"""

@@ -860,3 +860,32 @@ def test_state_of_another_order(dtype, master):
     with torch.no_grad():
         p.copy_(q)
     check_step(c, [p], 3, kw, 8, master)
+
+
+@pytest.mark.parametrize("where", ["cuda", "cpu"])
+def test_captured_step_follows_a_loaded_rate(where):
+    """and what is put into the group's tensor after the dictionary was loaded"""
+    def setup():
+        p = make([((600,), torch.float32)], seed=34)[0]
+        return p, AdamW([p], lr=torch.tensor(1e-2, device=DEV))
+    p, opt = setup()
+    q, ref = setup()
+    ref.step()
+    ref.param_groups[0]["lr"].fill_(0.25)
+    saved = copy.deepcopy(ref.state_dict())
+    saved["param_groups"][0]["lr"] = saved["param_groups"][0]["lr"].to(where)
+    opt.init_state()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    opt.load_state_dict(saved)
+    with torch.no_grad():
+        p.copy_(q)
+    for rate in (None, 0.5):
+        if rate:
+            opt.param_groups[0]["lr"].fill_(rate)
+            ref.param_groups[0]["lr"].fill_(rate)
+        graph.replay()
+        ref.step()
+        assert torch.equal(p, q)
+    assert int(opt.state[p]["step"]) == 3

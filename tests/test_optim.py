@@ -1,5 +1,6 @@
 """CPU checks of AdamW: refusals, the C entries' argument checks, the rounding
 noise of the 8-bit moments."""
+import copy
 import ctypes
 
 import numpy as np
@@ -331,3 +332,36 @@ def test_loaded_dictionary_leaves_a_groups_own_options(on_host):
     with pytest.raises(ValueError, match="exp_avg"):
         opt.load_state_dict(saved)
     assert opt.param_groups[1]["state_bits"] == 8
+
+
+def test_loaded_rate_goes_into_the_tensor(on_host):
+    """a rate on the optimizer's device stays the same tensor"""
+    p, q = leaf(5), leaf(6)
+    one, two = (torch.tensor(x) for x in (0.5, 0.25))
+    opt = AdamW([dict(params=[p], lr=one), dict(params=[q], lr=two)])
+    saved = copy.deepcopy(opt.state_dict())
+    for a, b in ((0.125, 0.0625), (torch.tensor(2.0), torch.tensor([4.0], dtype=torch.float64))):
+        saved["param_groups"][0]["lr"], saved["param_groups"][1]["lr"] = a, b
+        opt.load_state_dict(saved)
+        assert opt.param_groups[0]["lr"] is one and opt.param_groups[1]["lr"] is two
+        assert (float(one), float(two)) == (float(a), float(b))
+        saved["param_groups"][0]["lr"] = 9.0
+        assert float(one) == float(a)
+    # a number takes what comes
+    opt.param_groups[0]["lr"] = 0.5
+    opt.load_state_dict(saved)
+    assert opt.param_groups[0]["lr"] == 9.0
+    # refused: nothing is written
+    saved["param_groups"][1]["lr"] = torch.ones(2)
+    with pytest.raises(ValueError, match="one number"):
+        opt.load_state_dict(saved)
+    assert float(two) == 4.0
+    shared = torch.tensor(1.0)
+    opt = AdamW([dict(params=[p]), dict(params=[q])], lr=shared)
+    saved["param_groups"][1]["lr"] = 8.0
+    with pytest.raises(ValueError, match="share one lr"):
+        opt.load_state_dict(saved)
+    assert float(shared) == 1.0 and opt.param_groups[1]["lr"] is shared
+    saved["param_groups"][1]["lr"] = 9.0
+    opt.load_state_dict(saved)
+    assert float(shared) == 9.0 and opt.param_groups[0]["lr"] is shared
