@@ -19,6 +19,7 @@
 #include "flash_cqt_b200.h"
 
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <cstdint>
@@ -547,6 +548,8 @@ struct AdamWPlan {
     std::vector<int64_t> ends;           // of each group in todo
     std::vector<at::Tensor> keep;
     std::vector<const Slot*> stepped;    // the parameters behind todo
+    bool captured = false;               // a graph holds a step of this plan
+    std::vector<at::Tensor> graphed;     // what it addresses beside the plan's own
 
     static int32_t type_of(const at::Tensor& p) {
         return p.scalar_type() == at::kBFloat16 ? CQT_BF16
@@ -755,6 +758,13 @@ struct AdamWPlan {
         TORCH_CHECK_VALUE(!use_norm || (norm->get_device() == device && norm->numel() == 1 &&
                                         norm->scalar_type() == at::kFloat),
                           "grad_norm must hold one float32 number on cuda:", (int)device);
+        if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
+            // the graph addresses what this plan holds, the rates and the norm
+            captured = true;
+            if (use_norm) graphed.push_back(*norm);
+            for (auto gr : param_groups)
+                held.push_back(pybind11::reinterpret_borrow<pybind11::object>(item(gr.ptr(), "lr")));
+        }
         // autograd refuses a backward pass through values that it saved before
         // the step, as behind any operation in place
         for (const Slot* x : stepped)
@@ -953,6 +963,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         .def("last_heap", &Handle::last_heap);
     pybind11::class_<AdamWPlan>(m, "AdamWPlan")
         .def(pybind11::init<int, uintptr_t, uintptr_t, uintptr_t, pybind11::list, pybind11::dict>())
+        .def_readonly("captured", &AdamWPlan::captured)
         .def("fits", &AdamWPlan::fits)
         .def("step", &AdamWPlan::step);
     pybind11::class_<CacheHandle>(m, "CacheHandle")

@@ -147,7 +147,8 @@ class AdamW(torch.optim.Optimizer):
     made at a parameter's first step; before a step is captured it has to be
     there (``init_state()``, or a step).  ``load_state_dict`` (which also takes the
     state of ``torch.optim.AdamW``) writes into the state, and into a rate on the
-    device, that are there, so a captured step goes on from what was loaded.
+    device, that are there, so a captured step goes on from what was loaded (a
+    parameter that the dictionary has no state for goes back to zeros).
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *,
@@ -322,9 +323,13 @@ class AdamW(torch.optim.Optimizer):
                 for k, v in self.defaults.items():   # what is not said there stays
                     g.setdefault(k, old.get(k, v))
             rates = self._keep_rates(was)
-            new = {p: self._loaded(state_dict["state"][i], p, g)
-                   for old, g in zip(groups, self.param_groups)
-                   for i, p in zip(old["params"], g["params"]) if state_dict["state"].get(i)}
+            new = {}
+            for old, g in zip(groups, self.param_groups):
+                for i, p in zip(old["params"], g["params"]):
+                    if state_dict["state"].get(i):
+                        new[p] = self._loaded(state_dict["state"][i], p, g)
+                    elif before.get(p):   # it has taken no step: back to zeros
+                        new[p] = self._new_state(p, g)
         except Exception:
             self.param_groups[:] = was
             self.state.clear()
@@ -441,6 +446,8 @@ class AdamW(torch.optim.Optimizer):
         elif self._plan is None or not self._plan_step():
             # the first step, or states, parameters or groups were replaced
             self._lists()
+            if self._plan is not None and self._plan.captured:
+                self._retired.append(self._plan)   # a graph writes to its tensors
             self._plan = mod.AdamWPlan(
                 self._dev.index, *[_native.fn_address(n) for n in (
                     "cqt_grad_norm", "cqt_adamw_step", "cqt_last_error")],
@@ -495,6 +502,10 @@ class AdamW(torch.optim.Optimizer):
                     raise ValueError(f"grad_norm must hold one float32 number on {self._dev}")
                 _written([n])
             _written([t for _, p, s in keep for t in (p, *s.values())])
+            if torch.cuda.is_current_stream_capturing():
+                # the graph addresses these even when they have been replaced
+                self._retired.append((self.grad_norm, [g["lr"] for g in self.param_groups],
+                                      [(p, *s.values()) for _, p, s in keep]))
             self._launch(lists)
 
     def _launch(self, lists):

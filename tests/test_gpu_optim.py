@@ -3,6 +3,8 @@
 Tolerances: tests/plain_optim.py counts the roundings of each output; 16-bit
 parameters are rounded once more, by half a step of their type."""
 import copy
+import gc
+import weakref
 
 import numpy as np
 import pytest
@@ -889,3 +891,65 @@ def test_captured_step_follows_a_loaded_rate(where):
         ref.step()
         assert torch.equal(p, q)
     assert int(opt.state[p]["step"]) == 3
+
+
+@pytest.mark.parametrize("python", [False, True])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_step_goes_on_from_an_empty_state(bits, python, request):
+    """a dictionary that was saved before the first step"""
+    if python:
+        request.getfixturevalue("python_path")
+    def setup():
+        p = make([((600,), torch.float32)], seed=35)[0]
+        return p, AdamW([p], lr=1e-2, state_bits=bits)
+    p, opt = setup()
+    q, ref = setup()
+    empty = copy.deepcopy(opt.state_dict())
+    opt.step()
+    at = {k: t.data_ptr() for k, t in opt.state[p].items()}
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    opt.load_state_dict(empty)
+    with torch.no_grad():
+        p.copy_(q)
+    for _ in range(2):
+        graph.replay()
+        ref.step()
+    assert torch.equal(p, q) and int(opt.state[p]["step"]) == 2
+    assert {k: t.data_ptr() for k, t in opt.state[p].items()} == at
+    opt.step()   # a step of its own goes on from there
+    ref.step()
+    assert torch.equal(p, q) and int(opt.state[p]["step"]) == 3
+
+
+@pytest.mark.parametrize("python", [False, True])
+@pytest.mark.parametrize("capture", [False, True])
+def test_what_a_graph_writes_to_stays(capture, python, request):
+    """tensors that are replaced live on if, and only if, a graph addresses them"""
+    if python:
+        request.getfixturevalue("python_path")
+    p = make([((600,), torch.float32)], seed=36)[0]
+    # (a rate of the group's own: the constructor's default is kept by the class)
+    opt = AdamW([dict(params=[p], lr=torch.tensor(1e-2, device=DEV))], state_bits=8)
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    if capture:
+        with torch.cuda.graph(graph):
+            opt.step()
+    old = [weakref.ref(t) for k, t in opt.state[p].items() if k != "order"]
+    old.append(weakref.ref(opt.param_groups[0]["lr"]))
+    other = AdamW([make([((600,), torch.float32)], seed=37)[0]], lr=2e-2)
+    other.step()
+    opt.param_groups[0]["lr"] = 3e-2
+    opt.load_state_dict(other.state_dict())   # 32-bit moments
+    opt.step()
+    gc.collect()
+    assert opt.state[p]["exp_avg"].dtype == torch.float32 and opt.param_groups[0]["lr"] == 2e-2
+    # (the count has the same form in both and is used again)
+    assert [r() is not None for r in old] == [capture or k == 0 for k in range(len(old))]
+    if capture:
+        was = [t.clone() for t in opt.state[p].values()]
+        graph.replay()   # the old state's step, of the same parameter
+        assert torch.isfinite(p).all()
+        assert all(torch.equal(a, b) for a, b in zip(was[1:], list(opt.state[p].values())[1:]))

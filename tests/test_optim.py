@@ -365,3 +365,28 @@ def test_loaded_rate_goes_into_the_tensor(on_host):
     saved["param_groups"][1]["lr"] = 9.0
     opt.load_state_dict(saved)
     assert float(shared) == 9.0 and opt.param_groups[0]["lr"] is shared
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_that_is_not_loaded_goes_back_to_zeros(on_host, bits):
+    """in the tensors that are there: a captured step writes to them"""
+    p, q = leaf(300, dtype=torch.bfloat16), leaf(40)
+    opt = AdamW([p, q], state_bits=bits, master=True)
+    empty = opt.state_dict()
+    assert not empty["state"]
+    opt.load_state_dict(empty)
+    assert not opt.state          # nothing was there
+    opt.init_state()
+    fresh = copy.deepcopy(opt.state[p])
+    for t in opt.state[p].values():
+        if t is not opt.state[p].get("order"):
+            t.view(torch.uint8).random_(0, 100) if t.dim() else t.fill_(7)
+    was = dict(opt.state[p])
+    with torch.no_grad():
+        p.fill_(1.5)
+    opt.load_state_dict(empty)
+    assert set(opt.state) == {p, q}
+    for k, t in opt.state[p].items():
+        assert t is was[k]
+        want = torch.full((300,), 1.5) if k == "master" else fresh[k]
+        assert torch.equal(t.float(), want.float()), k
