@@ -307,24 +307,38 @@ class AdamW(torch.optim.Optimizer):
                 if not self.state.get(p):
                     self.state[p] = self._new_state(p, g)
 
-    @torch.no_grad()
     def load_state_dict(self, state_dict):
         """take over the options and the state of ``state_dict``; on a state that
         does not fit, ValueError, and the optimizer is as it was"""
-        groups = state_dict["param_groups"]
-        if any(g.get("amsgrad") or g.get("maximize") for g in groups):
-            raise ValueError("amsgrad and maximize do not exist here")
+        taken = {}
+
+        def take(_, dictionary):
+            # as the user's own hooks left it.  The base class would cast the state
+            # to the parameters' types: it only takes the groups
+            if any(g.get("amsgrad") or g.get("maximize") for g in dictionary["param_groups"]):
+                raise ValueError("amsgrad and maximize do not exist here")
+            taken.update(dictionary)
+            return dict(dictionary, state={})
         before, was = dict(self.state), [dict(g) for g in self.param_groups]
+        hooks = [self.register_load_state_dict_pre_hook(take),
+                 self.register_load_state_dict_post_hook(
+                     lambda opt: opt._take(taken, before, was), prepend=True)]
         try:
-            # the base class would cast the state to the parameters' types: it
-            # only takes the groups, the state is laid out here
-            super().load_state_dict(dict(state_dict, state={}))
+            super().load_state_dict(state_dict)
+        finally:
+            for h in hooks:
+                h.remove()
+
+    @torch.no_grad()
+    def _take(self, state_dict, before, was):
+        """the state of a dictionary whose groups the base class has taken over"""
+        try:
             for g, old in zip(self.param_groups, was):
                 for k, v in self.defaults.items():   # what is not said there stays
                     g.setdefault(k, old.get(k, v))
             rates = self._keep_rates(was)
             new = {}
-            for old, g in zip(groups, self.param_groups):
+            for old, g in zip(state_dict["param_groups"], self.param_groups):
                 for i, p in zip(old["params"], g["params"]):
                     if state_dict["state"].get(i):
                         new[p] = self._loaded(state_dict["state"][i], p, g)

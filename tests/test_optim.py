@@ -390,3 +390,41 @@ def test_state_that_is_not_loaded_goes_back_to_zeros(on_host, bits):
         assert t is was[k]
         want = torch.full((300,), 1.5) if k == "master" else fresh[k]
         assert torch.equal(t.float(), want.float()), k
+
+
+def test_load_hooks(on_host):
+    """hooks before a load may change what is loaded, those behind it see it"""
+    p = leaf(8)
+    opt = AdamW([p], lr=1e-2)
+    saved = torch_state((8,), lr=0.5)
+    m = saved["state"][0]["exp_avg"].clone()
+    seen = []
+
+    def returns(_, d):
+        state = {0: dict(d["state"][0], exp_avg=2 * d["state"][0]["exp_avg"])}
+        return dict(d, state=state, param_groups=[dict(d["param_groups"][0], lr=0.25)])
+
+    def changes(_, d):
+        d["state"] = {0: dict(d["state"][0], step=torch.tensor(40.0))}
+
+    def behind(o):
+        seen.append((float(o.state[p]["exp_avg"][0]), int(o.state[p]["step"]), o.param_groups[0]["lr"]))
+    handles = [opt.register_load_state_dict_pre_hook(returns),
+               opt.register_load_state_dict_pre_hook(changes, prepend=True),
+               opt.register_load_state_dict_post_hook(behind)]
+    for _ in range(2):
+        opt.load_state_dict(saved)
+    assert seen == [(2 * float(m[0]), 40, 0.25)] * 2
+    assert torch.equal(saved["state"][0]["exp_avg"], m) and saved["param_groups"][0]["lr"] == 0.5
+    bad = copy.deepcopy(saved)
+    bad["state"][0]["exp_avg_sq"] = torch.zeros(9)
+    with pytest.raises(ValueError, match="exp_avg_sq"):
+        opt.load_state_dict(bad)
+    handles[0].remove()   # (it gives one group for any number)
+    with pytest.raises(ValueError):
+        opt.load_state_dict(dict(saved, param_groups=saved["param_groups"] * 2))
+    assert len(seen) == 2   # nothing was loaded
+    for h in handles[1:]:
+        h.remove()
+    opt.load_state_dict(saved)
+    assert float(opt.state[p]["exp_avg"][0]) == float(m[0]) and opt.param_groups[0]["lr"] == 0.5
