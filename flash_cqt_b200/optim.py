@@ -319,7 +319,7 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("amsgrad and maximize do not exist here")
             taken.update(dictionary)
             return dict(dictionary, state={})
-        before, was = dict(self.state), [dict(g) for g in self.param_groups]
+        before, was = self.state, self.param_groups   # the base class brings its own
         hooks = [self.register_load_state_dict_pre_hook(take),
                  self.register_load_state_dict_post_hook(
                      lambda opt: opt._take(taken, before, was), prepend=True)]
@@ -345,9 +345,7 @@ class AdamW(torch.optim.Optimizer):
                     elif before.get(p):   # it has taken no step: back to zeros
                         new[p] = self._new_state(p, g)
         except Exception:
-            self.param_groups[:] = was
-            self.state.clear()
-            self.state.update(before)
+            self.state, self.param_groups = before, was
             raise
         for at, rate in rates.items():
             at.fill_(rate)

@@ -428,3 +428,24 @@ def test_load_hooks(on_host):
         h.remove()
     opt.load_state_dict(saved)
     assert float(opt.state[p]["exp_avg"][0]) == float(m[0]) and opt.param_groups[0]["lr"] == 0.5
+
+
+def test_refused_load_keeps_the_objects(on_host):
+    """a group or a state that a program holds is still the optimizer's own"""
+    p, q = leaf(8), leaf(9)
+    opt = AdamW([dict(params=[p], lr=0.5), dict(params=[q], state_bits=8)])
+    opt.init_state()
+    groups, state, own = opt.param_groups, opt.state, list(opt.param_groups)
+    options, entries = [dict(g) for g in own], {x: dict(s) for x, s in state.items()}
+    bad = copy.deepcopy(opt.state_dict())
+    bad["param_groups"][0]["lr"] = 0.125
+    bad["state"][1]["exp_avg_scale"] = torch.zeros(1)
+    with pytest.raises(ValueError, match="exp_avg_scale"):
+        opt.load_state_dict(bad)
+    assert opt.param_groups is groups and opt.state is state
+    assert all(a is b for a, b in zip(groups, own)) and [dict(g) for g in own] == options
+    assert state.keys() == entries.keys()
+    for x, s in state.items():
+        assert all(t is entries[x][k] for k, t in s.items())
+    opt.load_state_dict(copy.deepcopy(opt.state_dict()))
+    assert opt.param_groups[0]["lr"] == 0.5 and opt.state[p]["exp_avg"] is entries[p]["exp_avg"]
