@@ -1045,6 +1045,7 @@ int cqt_adamw_step(const cqt_adamw_tensor* tensors, int count, int state_bits,
     OptArgs o{};
     o.lr = a->lr;
     o.wd = a->weight_decay;
+    o.beta2 = a->beta2;
     o.ln1 = (float)std::log(a->beta1);   // -inf for 0: b^t is 0
     o.ln2 = (float)std::log(a->beta2);
     o.lr_dev = a->lr_dev;

@@ -272,7 +272,7 @@ struct OptTensor {
 };
 
 struct OptArgs {
-    double lr, wd;
+    double lr, wd, beta2;
     const float* lr_dev;       // not null: the rate is read from the device
     const double* norm;        // not null: gradients are scaled to max_norm
     double max_norm;

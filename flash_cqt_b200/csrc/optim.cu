@@ -377,7 +377,9 @@ struct Chunk {
     }
 };
 
-template <class T, int BITS, bool MASTER>
+// EXACT: the denominator and the quotient as the formula says, each rounded
+// once (see launch_adamw)
+template <class T, int BITS, bool MASTER, bool EXACT>
 __device__ __forceinline__ void update8(const OptTensor& t, const Chunk<T, BITS, MASTER>& c,
                                         const OptArgs& a, const StepScalars& s, unsigned key,
                                         int n, int vec, uint8_t* ms, uint8_t* vs) {
@@ -409,10 +411,18 @@ __device__ __forceinline__ void update8(const OptTensor& t, const Chunk<T, BITS,
         split(gi * gi * two(a.omb2), ra, rb);
         v[i] = __fadd_rn(v[i], ra);
         v[i + 1] = __fadd_rn(v[i + 1], rb);
+        if constexpr (EXACT) {
+#pragma unroll
+            for (int j = i; j < i + 2; ++j) {
+                const float d = __fadd_rn(__fmul_rn(__fsqrt_rn(v[j]), s.root), a.eps);
+                p[j] = __fadd_rn(__fmul_rn(p[j], s.decay), __fmul_rn(-s.rate, __fdiv_rn(m[j], d)));
+            }
+            continue;
+        }
         // root and reciprocal to 2^-23: their last bits are far below the
         // parameter's own, and correctly rounded ones took a third of all
         // instructions.  2^-126 under the root keeps what is subnormal
-        // from being read as 0 (above 2^-102 it changes nothing).
+        // from being read as 0; it moves the root by 2^-63 at most.
         float da, db;
         split(two(v[i], v[i + 1]) + two(0x1p-126f), ra, rb);
         split(two(root_of(ra), root_of(rb)) * two(s.root) + two(a.eps), da, db);
@@ -453,7 +463,7 @@ __device__ __forceinline__ void update8(const OptTensor& t, const Chunk<T, BITS,
 }
 
 // a chunk that the tensor ends in, or whose arrays are not aligned
-template <class T, int BITS, bool MASTER>
+template <class T, int BITS, bool MASTER, bool EXACT>
 __device__ __forceinline__ void update_part(const OptTensor& t, long long base, const OptArgs& a,
                                             const StepScalars& s, unsigned key, uint8_t* ms,
                                             uint8_t* vs) {
@@ -462,7 +472,7 @@ __device__ __forceinline__ void update_part(const OptTensor& t, long long base, 
     const int vec = n == 8 ? t.vec : 0;
     Chunk<T, BITS, MASTER> c;
     c.load(t, base, n, vec);
-    update8(t, c, a, s, key, n, vec, ms, vs);
+    update8<T, BITS, MASTER, EXACT>(t, c, a, s, key, n, vec, ms, vs);
 }
 
 constexpr int kWhole = 1 << 30;   // every thread has 8 aligned elements
@@ -504,7 +514,7 @@ struct TensorPlan {
     unsigned chunk0;
 };
 
-template <int N, class T, int BITS, bool MASTER>
+template <int N, class T, int BITS, bool MASTER, bool EXACT>
 __global__ void __launch_bounds__(kStepThreads<BITS>, kStepCtas<BITS>)
 adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ OptArgs a) {
     constexpr int kThreads = kStepThreads<BITS>, kChunk = kThreads * kLane;
@@ -595,8 +605,8 @@ adamw_kernel(const __grid_constant__ OptTable<N> tab, const __grid_constant__ Op
             const unsigned key = BITS == 8 ? mix32(q.key + (unsigned)(base >> 32)) : 0;
             uint8_t* ms = &scale[0][BITS == 8 ? k * kWarps + threadIdx.x / 32 : 0];
             uint8_t* vs = &scale[1][BITS == 8 ? k * kWarps + threadIdx.x / 32 : 0];
-            if (i & kWhole) update8(t, here, a, s, key, 8, 2, ms, vs);
-            else update_part<T, BITS, MASTER>(t, base, a, s, key, ms, vs);
+            if (i & kWhole) update8<T, BITS, MASTER, EXACT>(t, here, a, s, key, 8, 2, ms, vs);
+            else update_part<T, BITS, MASTER, EXACT>(t, base, a, s, key, ms, vs);
             here = next;
         }
         if constexpr (BITS == 8) {
@@ -758,31 +768,32 @@ unsigned resident_ctas(K kernel, int threads) {
     return (unsigned)(sms * per_sm);
 }
 
-template <int N, class T, int BITS, bool MASTER>
+template <int N, class T, int BITS, bool MASTER, bool EXACT>
 cudaError_t adamw_launch(const OptTensor* t, int count, const OptArgs& a, cudaStream_t s) {
     constexpr int kThreads = kStepThreads<BITS>;
     OptTable<N> tab;
     fill(&tab, t, count, kThreads * kLane);
-    static const unsigned most = resident_ctas(adamw_kernel<N, T, BITS, MASTER>, kThreads);
+    const auto kernel = adamw_kernel<N, T, BITS, MASTER, EXACT>;
+    static const unsigned most = resident_ctas(kernel, kThreads);
     // right behind the norm, the kernel may start on what the norm leaves free
-    return launch_pdl(a.behind_norm, adamw_kernel<N, T, BITS, MASTER>, dim3(opt_grid(tab.chunks, most)),
-                      dim3(kThreads), 0, s, tab, a);
+    return launch_pdl(a.behind_norm, kernel, dim3(opt_grid(tab.chunks, most)), dim3(kThreads), 0, s,
+                      tab, a);
 }
 
-template <int N, class T, bool MASTER>
+template <int N, bool EXACT, class T, bool MASTER>
 cudaError_t adamw_part(const OptTensor* t, int count, int bits, const OptArgs& a, cudaStream_t s) {
-    return bits == 8 ? adamw_launch<N, T, 8, MASTER>(t, count, a, s)
-                     : adamw_launch<N, T, 32, MASTER>(t, count, a, s);
+    return bits == 8 ? adamw_launch<N, T, 8, MASTER, EXACT>(t, count, a, s)
+                     : adamw_launch<N, T, 32, MASTER, EXACT>(t, count, a, s);
 }
 
-template <int N>
+template <int N, bool EXACT>
 cudaError_t adamw_typed(const OptTensor* t, int count, int bits, const OptArgs& a, cudaStream_t s) {
-    if (t->dtype == kOptF32) return adamw_part<N, float, false>(t, count, bits, a, s);
+    if (t->dtype == kOptF32) return adamw_part<N, EXACT, float, false>(t, count, bits, a, s);
     if (t->dtype == kOptBf16)
-        return t->master ? adamw_part<N, __nv_bfloat16, true>(t, count, bits, a, s)
-                         : adamw_part<N, __nv_bfloat16, false>(t, count, bits, a, s);
-    return t->master ? adamw_part<N, __half, true>(t, count, bits, a, s)
-                     : adamw_part<N, __half, false>(t, count, bits, a, s);
+        return t->master ? adamw_part<N, EXACT, __nv_bfloat16, true>(t, count, bits, a, s)
+                         : adamw_part<N, EXACT, __nv_bfloat16, false>(t, count, bits, a, s);
+    return t->master ? adamw_part<N, EXACT, __half, true>(t, count, bits, a, s)
+                     : adamw_part<N, EXACT, __half, false>(t, count, bits, a, s);
 }
 
 template <int N>
@@ -805,9 +816,18 @@ constexpr int kSmall = 12, kMiddle = 100;
 
 cudaError_t launch_adamw(const OptTensor* t, int count, int bits, OptArgs a, cudaStream_t s) {
     a.seed_key = mix32(a.seed_key);
-    if (count <= kSmall) return adamw_typed<kSmall>(t, count, bits, a, s);
-    if (count <= kMiddle) return adamw_typed<kMiddle>(t, count, bits, a, s);
-    return adamw_typed<kOptTensors>(t, count, bits, a, s);
+    // sqrt(v + 2^-126) is off by 2^-63 at most, so the denominator by 2^-63 /
+    // sqrt(1 - b2) (its bias correction at t = 1): under 2^-28 of eps, a sixteenth
+    // of a rounding, if eps is at least 2^-35 / sqrt(1 - b2) (9.2e-10 for b2 =
+    // 0.999).  Above 2^100 the reciprocal would come near to underflowing.  Other
+    // values of eps, which training has little use for, take the exact operations:
+    // as fast with 32-bit moments (302 us for 67 M floats), 234 us instead of 179
+    // with 8-bit ones, 310 instead of 221 for 96 M bf16 elements with those.
+    if (!(a.eps >= 0x1p-35 / sqrt(1.0 - a.beta2) && a.eps <= 0x1p100))
+        return adamw_typed<kOptTensors, true>(t, count, bits, a, s);
+    if (count <= kSmall) return adamw_typed<kSmall, false>(t, count, bits, a, s);
+    if (count <= kMiddle) return adamw_typed<kMiddle, false>(t, count, bits, a, s);
+    return adamw_typed<kOptTensors, false>(t, count, bits, a, s);
 }
 
 cudaError_t launch_grad_norm(const OptTensor* t, int count, double* partial, int* first, bool last,

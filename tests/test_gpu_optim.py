@@ -953,3 +953,43 @@ def test_what_a_graph_writes_to_stays(capture, python, request):
         graph.replay()   # the old state's step, of the same parameter
         assert torch.isfinite(p).all()
         assert all(torch.equal(a, b) for a, b in zip(was[1:], list(opt.state[p].values())[1:]))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("eps, size", [(0.0, 1e-17), (1e-30, 1e-17), (1e-18, 1e-17), (9e-10, 1e-17),
+                                       (1e-9, 1e-17), (1e-8, 1e-17), (0.0, 1.0), (1e-30, 1e-3),
+                                       (2e38, 1e17)])
+def test_any_eps(eps, size, dtype, bits):
+    """the formula's denominator for every eps that is accepted, and gradients as
+    small: v and g^2 stay normal numbers of float32, so every rounding is counted"""
+    if dtype == torch.float16 and size not in (1.0, 1e-3):
+        return   # (not numbers of that type)
+    ps = make([((700,), dtype), ((9, 31), dtype)], seed=38)
+    for p in ps:
+        with torch.no_grad():
+            p.zero_()   # the update is all there is
+        y = p.grad.float()
+        p.grad = (torch.sign(y) * (0.5 + y.abs()) * size).to(dtype)
+        assert (p.grad.float().abs() >= 0.49 * size).all()
+    opt = AdamW(ps, lr=1e-2, weight_decay=0.0, eps=eps, state_bits=bits, seed=2)
+    kw = dict(lr=1e-2, b1=0.9, b2=0.999, eps=eps, wd=0.0)
+    for t in (1, 2, 3):
+        check_step(opt, ps, t, kw, bits, seed=2)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_no_eps_at_the_border(bits):
+    """eps 0: a subnormal v, and 0 / 0 where there has been no gradient"""
+    p = torch.zeros(600, device=DEV, requires_grad=True)
+    p.grad = torch.full((600,), 1e-19, device=DEV)
+    p.grad[5] = p.grad[400] = 0.0
+    opt = AdamW([p], lr=1e-2, weight_decay=0.0, eps=0.0, state_bits=bits)
+    opt.step()
+    none = torch.zeros(600, dtype=torch.bool, device=DEV)
+    none[[5, 400]] = True
+    assert torch.isnan(p[none]).all()
+    # m / (1 - b1) = g and sqrt(v / (1 - b2)) = |g|: the update is the rate.  v =
+    # 1e-41 is rounded to a multiple of 2^-149, its root is off by half of that
+    off = (p.detach()[~none].double() / -1e-2 - 1).abs().max()
+    assert float(off) <= 0.5 * 2.0 ** -150 / 1e-41 * 1.01 + 31 * po.U
