@@ -45,7 +45,8 @@ class CoefCache:
     ``length`` (int64 [*lead], on the device) counts the slices that each
     stream has been given; ``codes`` [*lead, capacity, ncoef, 2] and ``scales``
     [*lead, capacity, ncoef / 16] are the store, in heap order.  A coefficient
-    is code * scale; a value that is not finite is held, and read, as NaN.
+    is code * scale; a value that is not finite is held, and read, as NaN.  To
+    restore a store that was saved, copy into the three.
 
     No gradient flows through the cache.  Calls on one cache must be ordered on
     one stream at a time; all of them may be captured into a graph.
@@ -75,10 +76,13 @@ class CoefCache:
             self.rows *= d
         store = (*self.lead, self.capacity)
         z = lambda *s: torch.zeros(*s, dtype=torch.uint8, device=self.dev)  # noqa: E731
-        self.codes = z(*store, self.ncoef, 2).view(dt)
-        self.scales = z(*store, self.ncoef // RUN).fill_(1).view(torch.float8_e8m0fnu)
-        self.length = torch.zeros(self.lead, dtype=torch.int64, device=self.dev)
+        self._codes = z(*store, self.ncoef, 2).view(dt)
+        self._scales = z(*store, self.ncoef // RUN).fill_(1).view(torch.float8_e8m0fnu)
+        self._length = torch.zeros(self.lead, dtype=torch.int64, device=self.dev)
         self._ws = z(max(4 * self.rows, 16))
+        # the same storage, kept whatever is done to the public tensors: a captured
+        # call addresses it
+        self._own = [t.detach() for t in (self.codes, self.scales, self.length)]
         i32 = ctypes.c_int32 * len(self.gspec)
         self._bands, self._lens = i32(*[b for b, _ in self.gspec]), i32(*[M for _, M in self.gspec])
         self._desc = _native.CqtCache(
@@ -92,6 +96,18 @@ class CoefCache:
                                               "cqt_last_error")],
             self.codes, self.scales, self.length, self._ws, self.capacity, self._format,
             [b for b, _ in self.gspec], [M for _, M in self.gspec], self.ngroups)
+
+    @property
+    def codes(self):
+        return self._codes
+
+    @property
+    def scales(self):
+        return self._scales
+
+    @property
+    def length(self):
+        return self._length
 
     def nbytes(self):
         """bytes of the store"""
@@ -125,6 +141,13 @@ class CoefCache:
                 raise ValueError(f"coefficient group {k} must be {want[0]}, got {shape}")
         return blocks, side, S
 
+    def _check_store(self):
+        d = self._desc
+        if [t.data_ptr() or None for t in (self.codes, self.scales, self.length)] != [
+                d.codes, d.scales, d.length]:
+            raise ValueError("the cache's codes, scales or length have another storage than they "
+                             "were made with (copy into them instead)")
+
     def _numbers(self, t, name):
         if t is None:
             return None
@@ -145,6 +168,7 @@ class CoefCache:
             return
         blocks, side, S = self._slices(blocks, side)   # refuses what does not fit
         counts = self._numbers(counts, "counts")
+        self._check_store()
         parts = (_native.CqtCachePart * len(self.gspec))()
         keep = []
         for k, (c, (b, M)) in enumerate(zip(blocks + side, self.gspec)):
@@ -178,6 +202,7 @@ class CoefCache:
         if self._h is not None:
             return self._h.window(n, dtype, _OUT[dtype], end)
         end = self._numbers(end, "end")
+        self._check_store()
         cplx = dtype == torch.complex64
         tail = () if cplx else (2,)
         out = torch.empty((self.rows * n * self.ncoef, *tail), dtype=dtype, device=self.dev)

@@ -799,6 +799,7 @@ using FnCacheWindow = decltype(&cqt_cache_window);
 
 struct CacheHandle {
     at::Tensor codes, scales, length, ws;
+    at::Tensor own[3];   // the same storage, kept whatever is done to those objects
     std::vector<int64_t> lead;
     std::vector<int32_t> bands, lens;
     int64_t ngroups, rows = 1, ncoef = 0;
@@ -820,6 +821,9 @@ struct CacheHandle {
           last_error(reinterpret_cast<FnLastError>(error)) {
         for (int64_t d : lead) rows *= d;
         for (size_t k = 0; k < bands.size(); ++k) ncoef += (int64_t)bands[k] * lens[k];
+        own[0] = codes.detach();
+        own[1] = scales.detach();
+        own[2] = length.detach();
         desc.codes = codes.data_ptr();
         desc.scales = static_cast<uint8_t*>(scales.data_ptr());
         desc.length = length.data_ptr<int64_t>();
@@ -837,6 +841,14 @@ struct CacheHandle {
         TORCH_CHECK(rc == 0, what, " failed (", rc, "): ", last_error());
     }
 
+    // the store's tensors are public, and their storage can be exchanged
+    void check_store() const {
+        TORCH_CHECK_VALUE(codes.data_ptr() == desc.codes && scales.data_ptr() == desc.scales &&
+                              length.data_ptr() == desc.length,
+                          "the cache's codes, scales or length have another storage than they "
+                          "were made with (copy into them instead)");
+    }
+
     const int64_t* numbers(const c10::optional<at::Tensor>& t, const char* name,
                            at::Tensor& hold) const {
         if (!t) return nullptr;
@@ -851,6 +863,7 @@ struct CacheHandle {
     // false (nothing done) for shapes that the caller has to sort out or refuse
     bool append(const std::vector<at::Tensor>& all, const c10::optional<at::Tensor>& counts) {
         at::NoGradGuard no_grad;
+        check_store();
         const size_t L = lead.size();
         if (all.size() != bands.size() || all[0].dim() != (int64_t)L + 2) return false;
         const int64_t S = all[0].size((int64_t)L + 1) / lens[0];
@@ -899,6 +912,7 @@ struct CacheHandle {
     pybind11::tuple window(int64_t n, at::ScalarType dtype, int type,
                            const c10::optional<at::Tensor>& end) {
         at::NoGradGuard no_grad;
+        check_store();
         at::Tensor hold;
         const int64_t* e = numbers(end, "end", hold);
         const bool cplx = dtype == at::kComplexFloat;

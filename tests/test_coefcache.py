@@ -134,3 +134,24 @@ def test_plain_quantiser(fmt, top):
     if fmt == "e4m3":   # torch's conversion agrees with the arithmetic
         t = torch.tensor(x / sc).to(torch.float8_e4m3fn).double().numpy()
         assert np.array_equal(t, c)
+
+
+@pytest.mark.parametrize("python", [False, True])
+@pytest.mark.parametrize("what", ["codes", "scales", "length"])
+def test_exchanged_store_is_refused(cqt, monkeypatch, what, python):
+    """kernels address the store that the cache was made with"""
+    import flash_cqt_b200.coefcache as module
+    monkeypatch.setattr(module, "_cuda_device", lambda d: torch.device("cpu"))
+    if python:
+        monkeypatch.setattr(_native, "_torchops", None)
+        monkeypatch.setattr(_native, "_torchops_tried", True)
+    c = CoefCache(cqt, (2, 1), 3)
+    with pytest.raises(AttributeError):
+        setattr(c, what, torch.zeros(1))
+    t = getattr(c, what)
+    t.data = t.data.clone()
+    with pytest.raises(ValueError, match="another storage"):
+        c.append(*blocks_of(c, 1))
+    with pytest.raises(ValueError, match="another storage"):
+        c.window(1)
+    assert CoefCache(cqt, (0,), 3).codes.numel() == 0

@@ -302,3 +302,35 @@ def test_refusals(banks):
     with pytest.raises(ValueError, match="end"):
         cache.window(1, end=torch.ones(1, dtype=torch.int64, device=DEV))
     assert int(cache.length.sum()) == 0
+
+
+@pytest.mark.parametrize("python", [False, True])
+def test_store_is_restored_by_copying(banks, python, monkeypatch):
+    """what was saved is copied into another cache; other storage is refused, and
+    a captured call goes on with the cache's own"""
+    if python:
+        from flash_cqt_b200 import _native
+        monkeypatch.setattr(_native, "_torchops", None)
+        monkeypatch.setattr(_native, "_torchops_tried", True)
+    cqt = banks["short"]
+    a, b = (CoefCache(cqt, (2,), 3, device=DEV) for _ in range(2))
+    src = to_blocks(heaps(2, 2, cqt.heap.ncoef, seed=6), cqt, (2,))
+    a.append(*src)
+    for k in ("codes", "scales", "length"):
+        x, y = getattr(a, k), getattr(b, k)
+        y.copy_(x)
+    want = from_blocks(*a.window(3), cqt, 3)
+    assert same(from_blocks(*b.window(3), cqt, 3), want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = b.window(3)
+    keep = b.codes.data
+    b.codes.data = torch.zeros_like(keep)
+    with pytest.raises(ValueError, match="another storage"):
+        b.window(3)
+    with pytest.raises(ValueError, match="another storage"):
+        b.append(*src)
+    del keep
+    torch.cuda.synchronize()
+    graph.replay()
+    assert same(from_blocks(*out, cqt, 3), want)
