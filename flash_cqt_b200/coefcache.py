@@ -185,6 +185,8 @@ class CoefCache:
             _native._check(_native.lib().cqt_cache_append(
                 ctypes.byref(self._desc), parts, S, counts.data_ptr() if counts is not None else None,
                 _raw_stream_of(self.dev.index)), "cqt_cache_append")
+        torch.autograd.graph.increment_version(
+            [t for t in (self.codes, self.scales, self.length) if not t.is_inference()])
 
     def window(self, n, dtype=torch.complex64, end=None):
         """slices [end - n, end) of every stream as (blocks, side) in the layout

@@ -472,7 +472,7 @@ struct Handle {
 using FnGradNorm = decltype(&cqt_grad_norm);
 using FnAdamw = decltype(&cqt_adamw_step);
 
-// a kernel is about to change a tensor that autograd may have saved
+// a kernel changes a tensor that autograd may have saved
 void written(const at::Tensor& t) {
     if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
@@ -906,6 +906,7 @@ struct CacheHandle {
         Ops::DeviceSwitch sw(device);
         check(append_fn(&desc, parts, (int)S, n, at::cuda::getCurrentCUDAStream(device).stream()),
               "cqt_cache_append");
+        for (const at::Tensor* t : {&codes, &scales, &length}) written(*t);
         return true;
     }
 

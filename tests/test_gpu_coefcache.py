@@ -334,3 +334,27 @@ def test_store_is_restored_by_copying(banks, python, monkeypatch):
     torch.cuda.synchronize()
     graph.replay()
     assert same(from_blocks(*out, cqt, 3), want)
+
+
+@pytest.mark.parametrize("python", [False, True])
+def test_append_is_seen_by_autograd(banks, python, monkeypatch):
+    """a backward pass through a store that has been appended to is refused"""
+    if python:
+        from flash_cqt_b200 import _native
+        monkeypatch.setattr(_native, "_torchops", None)
+        monkeypatch.setattr(_native, "_torchops_tried", True)
+    cqt = banks["short"]
+    cache = CoefCache(cqt, (2,), 3, device=DEV)
+    src = to_blocks(heaps(2, 1, cqt.heap.ncoef, seed=7), cqt, (2,))
+    cache.append(*src)
+    w = torch.ones(5, device=DEV, requires_grad=True)
+    y = w[cache.length].sum()          # the index is saved
+    cache.window(2)                    # (reading changes nothing)
+    y.backward()
+    assert w.grad.tolist() == [0, 2, 0, 0, 0]
+    y = w[cache.length].sum()
+    versions = [t._version for t in (cache.codes, cache.scales, cache.length)]
+    cache.append(*src)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    assert all(t._version > v for t, v in zip((cache.codes, cache.scales, cache.length), versions))
