@@ -185,7 +185,7 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"a tensor lr must hold one number, got {tuple(lr.shape)}")
             if lr.device.type == "cuda" and lr.dtype != torch.float32:
                 raise TypeError(f"a device lr must be float32, got {lr.dtype}")
-        elif not float(lr) >= 0:
+        if (not torch.is_tensor(lr) or lr.device.type == "cpu") and not float(lr) >= 0:
             raise ValueError(f"lr must not be negative, got {lr}")
         if not (0 <= b1 < 1 and 0 <= b2 < 1):
             raise ValueError(f"betas must lie in [0, 1), got {(b1, b2)}")

@@ -993,3 +993,19 @@ def test_no_eps_at_the_border(bits):
     # 1e-41 is rounded to a multiple of 2^-149, its root is off by half of that
     off = (p.detach()[~none].double() / -1e-2 - 1).abs().max()
     assert float(off) <= 0.5 * 2.0 ** -150 / 1e-41 * 1.01 + 31 * po.U
+
+
+@pytest.mark.parametrize("python", [False, True])
+def test_refused_host_rate_changes_nothing(python, request):
+    if python:
+        request.getfixturevalue("python_path")
+    ps = make([((50,), torch.float32), ((60,), torch.float32)], seed=39)
+    rate = torch.tensor(1e-2)
+    opt = AdamW([dict(params=[ps[0]]), dict(params=[ps[1]], lr=rate)], lr=1e-2)
+    opt.step()
+    was = [p.detach().clone() for p in ps]
+    rate.fill_(-1.0)
+    with pytest.raises(ValueError, match="lr"):
+        opt.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, was))
+    assert [int(opt.state[p]["step"]) for p in ps] == [1, 1]

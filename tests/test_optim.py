@@ -449,3 +449,12 @@ def test_refused_load_keeps_the_objects(on_host):
         assert all(t is entries[x][k] for k, t in s.items())
     opt.load_state_dict(copy.deepcopy(opt.state_dict()))
     assert opt.param_groups[0]["lr"] == 0.5 and opt.state[p]["exp_avg"] is entries[p]["exp_avg"]
+
+
+@pytest.mark.parametrize("lr", [-1.0, float("nan")])
+def test_rate_in_a_host_tensor_is_checked(lr):
+    """like a number: before anything is changed, not between two groups"""
+    with pytest.raises(ValueError, match="lr must not be negative"):
+        AdamW([leaf(3)], lr=torch.tensor(lr))
+    with pytest.raises(ValueError, match="lr must not be negative"):
+        AdamW._check_options(dict(lr=torch.tensor([lr], dtype=torch.float64), betas=(0.9, 0.9)))
