@@ -163,8 +163,9 @@ class CoefCache:
         side [*lead, 1, M] -- behind those that the streams have.  counts (int64
         [*lead] on the device): how many of the S slices each stream has
         (padded batches); the others are left out."""
-        if self._h is not None and side is not None and \
-                self._h.append([*blocks, *side], counts):
+        if side is not None:
+            blocks, side = list(blocks), list(side)   # looked at more than once
+        if self._h is not None and side is not None and self._h.append(blocks + side, counts):
             return
         blocks, side, S = self._slices(blocks, side)   # refuses what does not fit
         counts = self._numbers(counts, "counts")

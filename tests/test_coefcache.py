@@ -155,3 +155,16 @@ def test_exchanged_store_is_refused(cqt, monkeypatch, what, python):
     with pytest.raises(ValueError, match="another storage"):
         c.window(1)
     assert CoefCache(cqt, (0,), 3).codes.numel() == 0
+
+
+def test_blocks_from_an_iterator(cqt, monkeypatch):
+    """any iterable of blocks, also where the fast path leaves them to the other"""
+    import flash_cqt_b200.coefcache as module
+    monkeypatch.setattr(module, "_cuda_device", lambda d: torch.device("cpu"))
+    c = CoefCache(cqt, (2, 1), 3)
+    b, s = blocks_of(c, 1)
+    b[3] = b[3][..., :-1]
+    with pytest.raises(ValueError, match="group 3"):
+        c.append(iter(b), (x for x in s))
+    with pytest.raises(ValueError, match="side is needed"):
+        c.append(iter(b), None)

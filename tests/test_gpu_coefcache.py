@@ -358,3 +358,14 @@ def test_append_is_seen_by_autograd(banks, python, monkeypatch):
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
     assert all(t._version > v for t, v in zip((cache.codes, cache.scales, cache.length), versions))
+
+
+def test_lazy_views_from_an_iterator(banks):
+    """what the fast path does not take is appended all the same"""
+    cqt = banks["short"]
+    h = heaps(2, 1, cqt.heap.ncoef, seed=8)
+    blocks, side = to_blocks(h, cqt, (2,))
+    cache, ring = CoefCache(cqt, (2,), 2, device=DEV), pc.Ring(2, 2, cqt.heap.ncoef, "int8")
+    cache.append((b.conj().resolve_conj().conj() for b in blocks), iter(side))
+    ring.append(h)
+    check_store(cache, ring)
