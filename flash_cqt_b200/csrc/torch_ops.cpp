@@ -497,38 +497,44 @@ struct AdamWPlan {
         at::Tensor p;
         at::Tensor m, v, ms, vs, step, master;   // undefined: no state yet
         std::vector<int64_t> sizes, strides;     // of the parameter when it was checked
+        at::ScalarType type;
         cqt_adamw_tensor d{};
 
-        // whether the parameter has the memory order that its state was checked
-        // for: the codes of 8-bit moments are flat and do not show theirs
-        bool in_order() const {
-            if (p.sizes() != at::IntArrayRef(sizes)) return false;
+        // whether a tensor has the parameter's sizes and strides of that time (the
+        // codes of 8-bit moments are flat and do not show theirs)
+        bool in_order(const at::Tensor& t) const {
+            const at::IntArrayRef n = t.sizes(), s = t.strides();
+            if (n.size() != sizes.size()) return false;
             for (size_t k = 0; k < sizes.size(); ++k)
-                if (sizes[k] != 1 && p.stride((int64_t)k) != strides[k]) return false;
+                if (n[k] != sizes[k] || (s[k] != strides[k] && n[k] != 1)) return false;
             return true;
         }
+        // plain memory on the device: usually seen by the same set of dispatch keys
+        // as a tensor that is known to be
+        static bool plain(const at::Tensor& t, at::ScalarType type, c10::DeviceIndex device,
+                          const at::Tensor* known = nullptr) {
+            return t.defined() && t.scalar_type() == type && t.get_device() == device &&
+                   ((known && t.key_set() == known->key_set()) ||
+                    (t.layout() == at::kStrided && !t.is_conj() && !t.is_neg()));
+        }
 
-        // whether the state is what the kernels take for the parameter
-        bool fits(int bits) const {
-            const auto at_home = [&](const at::Tensor& t, at::ScalarType type) {
-                return t.defined() && t.scalar_type() == type && t.layout() == at::kStrided &&
-                       t.get_device() == p.get_device() && !t.is_conj() && !t.is_neg();
-            };
+        // whether the state is what the kernels take for the (plain) parameter
+        bool fits(int bits, c10::DeviceIndex device) const {
             const auto like_p = [&](const at::Tensor& t, at::ScalarType type) {
-                return at_home(t, type) && t.sizes() == p.sizes() && same_order(t, p);
+                return plain(t, type, device, &p) && in_order(t);
             };
             const auto flat = [&](const at::Tensor& t, at::ScalarType type, int64_t n) {
-                return at_home(t, type) && t.numel() == n && t.is_contiguous();
+                return plain(t, type, device, &p) && t.numel() == n && t.is_contiguous();
             };
-            if (!at_home(step, at::kLong) || step.numel() != 1) return false;
+            if (!plain(step, at::kLong, device, &p) || step.numel() != 1) return false;
             if (master.defined() && !like_p(master, at::kFloat)) return false;
             if (bits == 8) {
                 const int64_t blocks = (d.numel + 255) / 256;
                 return flat(m, at::kFloat8_e4m3fn, d.numel) && flat(v, at::kFloat8_e5m2, d.numel) &&
                        flat(ms, at::kFloat8_e8m0fnu, blocks) && flat(vs, at::kFloat8_e8m0fnu, blocks);
             }
-            const at::ScalarType type = p.is_complex() ? at::kComplexFloat : at::kFloat;
-            return like_p(m, type) && like_p(v, type);
+            const at::ScalarType moments = type == at::kComplexFloat ? type : at::kFloat;
+            return like_p(m, moments) && like_p(v, moments);
         }
     };
     struct Group {
@@ -588,6 +594,7 @@ struct AdamWPlan {
                 out.slots.emplace_back();
                 Slot& s = out.slots.back();
                 s.p = p.cast<at::Tensor>();
+                s.type = s.p.scalar_type();
                 s.sizes = s.p.sizes().vec();
                 s.strides = s.p.strides().vec();
                 s.d.ordinal = ordinal++;
@@ -662,12 +669,9 @@ struct AdamWPlan {
                                   "a gradient must be ", p.scalar_type(), " ", p.sizes(), " on ",
                                   p.device(), ", got ", grad.scalar_type(), " ", grad.sizes(),
                                   " on ", grad.device());
-                // the parameter's storage may have been exchanged
-                const int64_t n = p.numel() * (p.is_complex() ? 2 : 1);
-                if (n != s.d.numel || type_of(p) != s.d.dtype || p.get_device() != device ||
-                    !p.is_non_overlapping_and_dense() || p.is_conj() || p.is_neg())
+                // the storage of a parameter or of a state may have been exchanged
+                if (!Slot::plain(p, s.type, device) || !s.in_order(p) || !s.fits(g.bits, device))
                     return false;
-                if (!s.in_order() || !s.fits(g.bits)) return false;
                 at::Tensor use = grad;
                 if (grad.is_conj() || grad.is_neg() || !same_order(grad, p)) {
                     use = at::empty_like(p).copy_(grad);
@@ -710,6 +714,20 @@ struct AdamWPlan {
         if (x == -1.0 && PyErr_Occurred()) throw pybind11::error_already_set();
         return x;
     }
+
+    // Autograd refuses a backward pass through values that it saved before a step,
+    // as behind any operation in place: marks what the launches write, behind
+    // them (the GPU is at work meanwhile) and also behind one that failed.
+    struct Marks {
+        const AdamWPlan& plan;
+        const at::Tensor* norm;
+        ~Marks() {
+            for (const Slot* x : plan.stepped)
+                for (const at::Tensor* t : {&x->p, &x->m, &x->v, &x->ms, &x->vs, &x->step, &x->master})
+                    written(*t);
+            if (norm) written(*norm);
+        }
+    };
 
     // one step; false (nothing done) when the plan does not fit any more
     bool step(pybind11::list param_groups, pybind11::dict state, pybind11::object max_norm,
@@ -765,12 +783,7 @@ struct AdamWPlan {
             for (auto gr : param_groups)
                 held.push_back(pybind11::reinterpret_borrow<pybind11::object>(item(gr.ptr(), "lr")));
         }
-        // autograd refuses a backward pass through values that it saved before
-        // the step, as behind any operation in place
-        for (const Slot* x : stepped)
-            for (const at::Tensor* t : {&x->p, &x->m, &x->v, &x->ms, &x->vs, &x->step, &x->master})
-                written(*t);
-        if (use_norm) written(*norm);
+        const Marks marks{*this, use_norm ? &*norm : nullptr};
         if (use_norm) {
             check(norm_fn(todo.data(), (int)todo.size(), norm->data_ptr<float>(), ws.data_ptr(),
                           (size_t)ws.numel(), stream),

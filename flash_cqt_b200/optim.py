@@ -164,6 +164,7 @@ class AdamW(torch.optim.Optimizer):
     def _reset(self):
         self._dev = self._ws = self._plan = self.grad_norm = None
         self._retired = []
+        self._need = None, 0   # a number of tensors and the workspace for it
 
     def __getstate__(self):
         return dict(super().__getstate__(), max_norm=self.max_norm, seed=self.seed)
@@ -422,7 +423,9 @@ class AdamW(torch.optim.Optimizer):
 
     def _workspace(self, count):
         """grow-only; an outgrown one is kept: a captured graph may address it"""
-        need = _native.lib().cqt_adamw_workspace_bytes(count)
+        if self._need[0] != count:
+            self._need = count, _native.lib().cqt_adamw_workspace_bytes(count)
+        need = self._need[1]
         if self._ws is None or self._ws.numel() < need or (
                 self.max_norm is not None and self.grad_norm is None):
             if torch.cuda.is_current_stream_capturing():
