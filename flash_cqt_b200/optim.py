@@ -36,7 +36,7 @@ def _fills(shape, strides):
 
 def _dense(t):
     """whether the elements fill one stretch of memory, in any order of dims"""
-    return _fills(t.shape, t.stride())
+    return t.is_contiguous() or _fills(t.shape, t.stride())
 
 
 def _same_order(a, b):
@@ -46,13 +46,13 @@ def _same_order(a, b):
 
 def _order(p):
     """the memory order of a dense tensor: its sizes over its strides"""
-    return torch.tensor([list(p.shape), list(p.stride())], dtype=torch.int64)
+    return torch.tensor([*p.shape, *p.stride()], dtype=torch.int64).view(2, p.dim())
 
 
 def _ordered_like(order, p):
     shape, strides = order.tolist()
-    return shape == list(p.shape) and all(
-        a == b for a, b, n in zip(strides, p.stride(), shape) if n != 1)
+    return shape == list(p.shape) and (strides == list(p.stride()) or all(
+        a == b for a, b, n in zip(strides, p.stride(), shape) if n != 1))
 
 
 def _values8(codes, scales):
@@ -460,7 +460,7 @@ class AdamW(torch.optim.Optimizer):
             self._python_step()
         elif self._plan is None or not self._plan_step():
             # the first step, or states, parameters or groups were replaced
-            self._lists()
+            self._lists(plan=True)
             if self._plan is not None and self._plan.captured:
                 self._retired.append(self._plan)   # a graph writes to its tensors
             self._plan = mod.AdamWPlan(
@@ -477,10 +477,10 @@ class AdamW(torch.optim.Optimizer):
                                self.grad_norm)
 
     @torch.no_grad()
-    def _lists(self):
+    def _lists(self, plan=False):
         """the tensors of every group that have gradients, as the library takes
         them (states are made and checked), and (gradient or its copy, parameter,
-        state) of each"""
+        state) of each; for a plan, which looks at the rest itself, states only"""
         lists, keep = [], []
         first = 0
         for g in self.param_groups:
@@ -491,13 +491,16 @@ class AdamW(torch.optim.Optimizer):
                     continue
                 self._check_param(p)   # its storage may have been exchanged
                 s = self.state.get(p)
-                if not s:
+                if s:
+                    self._check_state(s, p, g)
+                else:
                     s = self.state[p] = self._new_state(p, g)
+                if g["state_bits"] == 8 and "order" not in s:
+                    s["order"] = _order(p)
+                if plan:
+                    continue
                 grad = self._grad(p)
                 keep.append((grad, p, s))
-                self._check_state(s, p, g)
-                if g["state_bits"] == 8:
-                    s.setdefault("order", _order(p))
                 at = lambda k: s[k].data_ptr() if k in s else None  # noqa: E731
                 todo.append(_native.CqtAdamwTensor(
                     p.data_ptr(), grad.data_ptr(), at("master") if g["master"] else None,
