@@ -39,8 +39,8 @@ class CoefCache:
 
     cqt: the transform that the coefficients come from; lead: the leading
     dimensions of its blocks, e.g. (B, C).  ``fmt`` is "int8" (steps of 1/127
-    of the largest of 16 neighbours) or "e4m3" (3 bits behind the leading one,
-    down to 2^-15 of it).  Slice k of a stream lies in slot k mod capacity.
+    to 1/64 of the largest of 16 neighbours: the scale is a power of two) or
+    "e4m3" (3 bits behind the leading one, down to about 2^-14 of it).  Slice k of a stream lies in slot k mod capacity.
 
     ``length`` (int64 [*lead], on the device) counts the slices that each
     stream has been given; ``codes`` [*lead, capacity, ncoef, 2] and ``scales``

@@ -23,9 +23,11 @@
 // before the launch, and a captured graph holds it.
 //
 // Every byte is touched once, so DRAM bounds the step: 144 M bf16 elements with
-// a master copy 660 us (6.1 TB/s), 67 M floats with 8-bit moments 180 us (6.0
-// TB/s).  16-bit parameters with 8-bit moments move 10 bytes for 57 instructions
-// an element and stay at 4.3 TB/s (96 M elements, 225 us).
+// a master copy 660 us (6.1 TB/s), 67 M floats with 8-bit moments 180 to 193 us
+// (6.0 to 5.6 TB/s, from one GPU to another).  16-bit parameters with 8-bit moments
+// move 10 bytes for 57 instructions an element, which would take as long as the
+// bytes if they were issued without a pause, and stay at 4.3 TB/s (96 M elements,
+// 221 us).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -45,7 +47,9 @@ static_assert(32 * kLane == kOptBlock, "a warp is one block");
 // CTA sizes.  Measured with 8-bit moments, 67 M float and 96 M bf16 elements: 181
 // and 225 us with 7 CTAs of 128 threads an SM (72 registers), 190 and 233 with 3
 // of 256, 192 and 233 with 4 of 192, 210 and 224 with 4 of 224, 221 and 315 with
-// 4 of 256 (64 registers, spilled).  32-bit moments move more bytes an element
+// 4 of 256 (64 registers, spilled).  A table of more than 100 tensors takes 42 KB of
+// shared memory and leaves room for 5 of the 7: 25 M bf16 elements with clipping
+// 80 us as 100 tensors, 125 as 101.  32-bit moments move more bytes an element
 // and want fewer threads: 144 M bf16 elements with a master copy 660 us with 16
 // warps an SM, 675 with 24, 750 with 32.
 template <int BITS>

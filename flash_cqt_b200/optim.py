@@ -134,7 +134,9 @@ class AdamW(torch.optim.Optimizer):
     laid out anew when it is loaded, which rounds only what is small beside its
     new neighbours.  They are rounded stochastically by a
     hash of (``seed``, t, the parameter's number, element): the same run gives
-    the same bits.  ``master=True`` keeps a 32-bit copy of a 16-bit parameter,
+    the same bits.  A first moment below 2^-6 of its block's scale is held as 0: an
+    element whose gradients stay under about 5e-5 of the largest in its block hardly
+    moves (3e-5 of it: 6 % of the update that 32-bit moments give; 1e-4: all of it).  ``master=True`` keeps a 32-bit copy of a 16-bit parameter,
     which is then its rounding; without it a 16-bit parameter loses updates
     below half a step of its type.  Both may differ between parameter groups.
 
@@ -146,7 +148,8 @@ class AdamW(torch.optim.Optimizer):
     Steps of one optimizer must be ordered on one stream at a time.  State is
     made at a parameter's first step; before a step is captured it has to be
     there (``init_state()``, or a step).  ``load_state_dict`` (which also takes the
-    state of ``torch.optim.AdamW``) writes into the state, and into a rate on the
+    state of ``torch.optim.AdamW``, for 32-bit moments: there is no conversion
+    between the widths) writes into the state, and into a rate on the
     device, that are there, so a captured step goes on from what was loaded (a
     parameter that the dictionary has no state for goes back to zeros).
     """
