@@ -367,7 +367,7 @@ class SliceStream:
         self.kf = self.kb = 0
         if int(history) < 0:
             raise ValueError(f"history must not be negative, got {history}")
-        self.cache = CoefCache(sliced, self.lead, history, history_format, dev) if history else None
+        self._cache = CoefCache(sliced, self.lead, history, history_format, dev) if history else None
         held = se.group_views(self.coef, self.lead, 1)
 
         def fwd_body(s0):
@@ -400,6 +400,11 @@ class SliceStream:
                         body(s0)
                     lst.append(g)
         self.reset()
+
+    @property
+    def cache(self):
+        """the history (None without one); the graphs write to this one"""
+        return self._cache
 
     def reset(self):
         """start a new stream (the state buffers are cleared)"""

@@ -146,3 +146,14 @@ def test_whole_step_in_a_graph(sliced):
     for g, w in zip(gains, want):
         assert torch.equal(g.detach(), w)
     assert int(opt.state[gains[0]]["step"]) == 4
+
+
+def test_history_is_the_streams_own(sliced):
+    """the graphs write to the cache that they were captured with"""
+    st = sliced.streamer((1, 1), history=2)
+    with pytest.raises(AttributeError):
+        st.cache = CoefCache(sliced, (1, 1), 2)
+    assert sliced.streamer((1, 1)).cache is None
+    x = torch.randn(1, 1, sliced.hop, device=DEV)
+    st.fwd(x)
+    assert int(st.cache.length) == 1 and st.past(1)[0][0].abs().max() > 0
