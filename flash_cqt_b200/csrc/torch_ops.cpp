@@ -615,10 +615,32 @@ struct AdamWPlan {
                     s.vs = get("exp_avg_sq_scale");
                 }
                 if (out.master && s.d.dtype != CQT_F32) s.master = get("master");
+                // (a parameter without a gradient has not been checked by the caller)
+                if (!plan_takes(s, out.bits, get("order")))
+                    s.m = s.v = s.ms = s.vs = s.step = s.master = at::Tensor();
             }
         }
         walk(state.ptr(), seen);
         for (PyObject* o : seen) held.push_back(pybind11::reinterpret_borrow<pybind11::object>(o));
+    }
+
+    // whether a parameter is what the kernels take, in the memory order of its state
+    // (of 8-bit moments: the sizes over the strides; those of a contiguous parameter
+    // if nothing says it)
+    bool plan_takes(const Slot& s, int bits, const at::Tensor& order) const {
+        if (s.d.dtype < 0 || !Slot::plain(s.p, s.type, device) || !s.p.is_non_overlapping_and_dense())
+            return false;
+        if (bits != 8) return true;   // their own order is compared at each step
+        if (!order.defined()) return s.p.is_contiguous();
+        const int64_t dims = s.p.dim();
+        if (order.scalar_type() != at::kLong || order.dim() != 2 || order.size(0) != 2 ||
+            order.size(1) != dims)
+            return false;
+        const at::Tensor host = order.cpu().contiguous();
+        const int64_t* n = host.data_ptr<int64_t>();
+        for (int64_t k = 0; k < dims; ++k)
+            if (n[k] != s.sizes[k] || (n[dims + k] != s.strides[k] && n[k] != 1)) return false;
+        return true;
     }
 
     // whether what this was built from is still what the optimizer holds

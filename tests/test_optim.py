@@ -465,3 +465,34 @@ def test_rate_in_a_host_tensor_is_checked(lr):
         AdamW([leaf(3)], lr=torch.tensor(lr))
     with pytest.raises(ValueError, match="lr must not be negative"):
         AdamW._check_options(dict(lr=torch.tensor([lr], dtype=torch.float64), betas=(0.9, 0.9)))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_parameters_without_gradients_are_checked_too(on_host, bits):
+    """a plan that is made while a parameter has none does not take it as it is
+    then: its order may have changed since its state was made"""
+    p, q = leaf(6, 40), leaf(5)
+    opt = AdamW([p, q], state_bits=bits)
+    opt.init_state()
+    q.grad = torch.ones(5)
+    was = p.data
+    for other in (was.t().contiguous().t(), torch.zeros(6, 80)[:, ::2], torch.zeros(1).expand(6, 40),
+                  was.t().contiguous(), was.double()):
+        p.data = other
+        plan = plans().AdamWPlan(-1, 0, 0, 0, opt.param_groups, opt.state)
+        assert plan.fits(opt.param_groups, opt.state)        # nothing is done with it
+        p.grad = torch.empty_strided(p.shape, p.stride(), dtype=p.dtype)
+        assert not plan.fits(opt.param_groups, opt.state)
+        p.grad = None
+        p.data = was
+    plan = plans().AdamWPlan(-1, 0, 0, 0, opt.param_groups, opt.state)
+    p.grad = torch.ones(6, 40)
+    assert plan.fits(opt.param_groups, opt.state)
+    if bits == 8:   # without the record: a contiguous parameter's
+        del opt.state[p]["order"]
+        plan = plans().AdamWPlan(-1, 0, 0, 0, opt.param_groups, opt.state)
+        assert plan.fits(opt.param_groups, opt.state)
+        for bad in (torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 2), torch.zeros(4).long()):
+            opt.state[p]["order"] = bad
+            plan = plans().AdamWPlan(-1, 0, 0, 0, opt.param_groups, opt.state)
+            assert not plan.fits(opt.param_groups, opt.state)
