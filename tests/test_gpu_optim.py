@@ -1009,3 +1009,24 @@ def test_refused_host_rate_changes_nothing(python, request):
         opt.step()
     assert all(torch.equal(p, q) for p, q in zip(ps, was))
     assert [int(opt.state[p]["step"]) for p in ps] == [1, 1]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_through_a_file(bits):
+    """saved and loaded to the device, the record of the order with it, into a
+    parameter in another order"""
+    import io
+    p = make([((4, 6, 70), torch.bfloat16)], seed=40)[0]
+    a = AdamW([p], lr=1e-2, state_bits=bits, master=True)
+    a.step()
+    f = io.BytesIO()
+    torch.save(a.state_dict(), f)
+    q = p.detach().transpose(0, 2).contiguous().transpose(0, 2).requires_grad_()
+    q.grad = torch.empty_like(q).copy_(p.grad)
+    b = AdamW([q], lr=1e-2, state_bits=bits, master=True)
+    for where in (DEV, "cpu"):
+        f.seek(0)
+        b.load_state_dict(torch.load(f, map_location=where, weights_only=True))
+    assert torch.equal(b.state[q]["master"], a.state[p]["master"])
+    assert b.state[q]["master"].stride() == q.stride()
+    check_step(b, [q], 2, dict(lr=1e-2, b1=0.9, b2=0.999, eps=1e-8, wd=1e-2), bits, True)
